@@ -94,6 +94,10 @@ SYMBOLS = {
     "dlp_activation_fwd": (_i, [_fp, _fp, _sz, _i, _vp]),
     "dlp_softmax_fwd": (_i, [_fp, _fp, _i, _i, _i, _i, _vp]),
     "dlp_batchnorm_inference_fwd": (_i, [_fp, _fp, _i, _i, _i, _f, _fp, _fp, _fp, _fp, _vp]),
+    "dlp_rms_norm_fwd": (_i, [_vp, _ll, _vp, _ll, _vp, _ll, _vp, _i, _vp, _ll, _i, _vp, _ll, _i, _i, _f, _vp]),
+    "dlp_quantize_fwd": (_i, [_vp, _ll, _i, _i, _vp, _ll, _vp, _ll, _i, _i, _i, _vp]),
+    "dlp_scaled_ip_fwd": (_i, [_vp, _ll, _vp, _ll, _vp, _ll, _vp, _ll, _vp, _vp, _ll, _i, _i, _i, _i, _i, _vp]),
+    "dlp_sample_fwd": (_i, [_vp, _ll, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
 }
 
 _lib = None
@@ -383,3 +387,94 @@ def batchnorm_inference(x, y, mean, var, gamma=None, beta=None, eps=1e-5, stream
         plane *= s
     check(lib().dlp_batchnorm_inference_fwd(_ptr(x), _ptr(y), x.shape[0], x.shape[1], plane, eps, _ptr(mean), _ptr(var), _ptr(gamma),
                                             _ptr(beta), _stream(stream)))
+
+
+# ---- operators with typed operands: from a hidden state to a token ---------------------------------
+GATES = {"none": 0, "silu": 1, "gelu": 2}
+TYPES = {"float32": 0, "float16": 1, "bfloat16": 2, "float8_e4m3fn": 3}
+SCALE_BLOCK = 128
+SAMPLE_MAX_CLASSES = 1 << 22
+_type_codes = {}
+
+
+def _type(t):
+    """DLP_TYPE_* of a tensor."""
+    code = _type_codes.get(t.dtype)
+    if code is None:
+        code = TYPES.get(str(t.dtype).replace("torch.", ""))
+        if code is None:
+            raise ValueError("fp32, fp16, bf16 or e4m3 tensors expected, not %s" % t.dtype)
+        _type_codes[t.dtype] = code
+    return code
+
+
+def _typed(t, code, shape, name, device):
+    """(address, row stride) of a vector or matrix of this shape, with unit stride along its rows, on the current device."""
+    if tuple(t.shape) != shape:
+        raise ValueError("%s: expected shape %s, not %s" % (name, list(shape), list(t.shape)))
+    if code >= 0 and _type(t) != code:
+        raise ValueError("%s: another type was expected than %s" % (name, t.dtype))
+    if t.get_device() != device:
+        raise ValueError("%s is not on the current device" % name)
+    stride = t.stride()
+    if stride[-1] != 1 and shape[-1] > 1:
+        raise ValueError("%s: rows must be contiguous" % name)
+    return t.data_ptr(), (stride[0] if len(shape) > 1 else 0)
+
+
+def _device():
+    import torch
+    return torch.cuda.current_device()
+
+
+def rms_norm(x, weight, y, residual=None, total=None, scales=None, eps=1e-6, stream=None):
+    """y = h / sqrt(mean(h^2) + eps) * weight with h = x + residual; total (optional) receives h.  An e4m3 y comes with scales
+    [ceil(cols / 128), rows]."""
+    rows, cols = x.shape
+    dev, t, yt = _device(), _type(x), _type(y)
+    xp, xs = _typed(x, t, (rows, cols), "x", dev)
+    wp, _ = _typed(weight, t, (cols,), "weight", dev)
+    yp, ys = _typed(y, yt, (rows, cols), "y", dev)
+    rp, rs = _typed(residual, t, (rows, cols), "residual", dev) if residual is not None else (None, 0)
+    tp, ts = _typed(total, t, (rows, cols), "total", dev) if total is not None else (None, 0)
+    sp, ss = _typed(scales, 0, (-(-cols // SCALE_BLOCK), rows), "scales", dev) if scales is not None else (None, 0)
+    check(lib().dlp_rms_norm_fwd(xp, xs, rp, rs, tp, ts, wp, t, yp, ys, yt, sp, ss, rows, cols, eps, _stream(stream)))
+
+
+def quantize(x, q, scales, gate="none", block_rows=1, stream=None):
+    """q [rows, cols] (e4m3) and scales: the 8-bit form of x, or of act(a) * b for x = [a | b] (gate "silu" or "gelu").  block_rows 1: scales
+    [ceil(cols / 128), rows]; 128: [ceil(rows / 128), ceil(cols / 128)]."""
+    rows, cols = q.shape
+    dev, t, g = _device(), _type(x), GATES[gate]
+    xp, xs = _typed(x, t, (rows, 2 * cols if g else cols), "x", dev)
+    qp, qs = _typed(q, TYPES["float8_e4m3fn"], (rows, cols), "q", dev)
+    blocks = -(-cols // SCALE_BLOCK)
+    sp, ss = _typed(scales, 0, (blocks, rows) if block_rows == 1 else (-(-rows // SCALE_BLOCK), blocks), "scales", dev)
+    check(lib().dlp_quantize_fwd(xp, xs, t, g, qp, qs, sp, ss, block_rows, rows, cols, _stream(stream)))
+
+
+def scaled_inner_product(x, x_scales, w, w_scales, y, bias=None, activation="identity", stream=None):
+    """y = act(x * w^T + bias) for 8-bit x [rows, inputs] in blocks of one row and w [outputs, inputs] in blocks of 128 x 128."""
+    (rows, inputs), outputs = x.shape, w.shape[0]
+    dev, e4m3, yt, blocks = _device(), TYPES["float8_e4m3fn"], _type(y), -(-inputs // SCALE_BLOCK)
+    xp, xs = _typed(x, e4m3, (rows, inputs), "x", dev)
+    xsp, xss = _typed(x_scales, 0, (blocks, rows), "x_scales", dev)
+    wp, ws = _typed(w, e4m3, (outputs, inputs), "w", dev)
+    wsp, wss = _typed(w_scales, 0, (-(-outputs // SCALE_BLOCK), blocks), "w_scales", dev)
+    yp, ys = _typed(y, yt, (rows, outputs), "y", dev)
+    bp = _typed(bias, 0, (outputs,), "bias", dev)[0] if bias is not None else None
+    check(lib().dlp_scaled_ip_fwd(xp, xs, xsp, xss, wp, ws, wsp, wss, bp, yp, ys, yt, _act(activation), rows, inputs, outputs, _stream(stream)))
+
+
+def sample(logits, u, tokens, temperature=None, top_k=None, top_p=None, min_p=None, stream=None):
+    """tokens [rows] (int32): a class drawn from each row of logits with the row's random number u in [0, 1); -1 where every logit is
+    masked.  Settings are per-row vectors or None."""
+    import torch
+    rows, classes = logits.shape
+    dev, t = _device(), _type(logits)
+    lp, ls = _typed(logits, t, (rows, classes), "logits", dev)
+    if tokens.dtype != torch.int32 or (top_k is not None and top_k.dtype != torch.int32):
+        raise ValueError("tokens and top_k are int32")
+    row = [None if v is None else _typed(v, code, (rows,), name, dev)[0] for v, code, name in (
+        (temperature, 0, "temperature"), (top_k, -1, "top_k"), (top_p, 0, "top_p"), (min_p, 0, "min_p"), (u, 0, "u"), (tokens, -1, "tokens"))]
+    check(lib().dlp_sample_fwd(lp, ls, t, rows, classes, *row, _stream(stream)))

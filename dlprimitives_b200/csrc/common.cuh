@@ -68,6 +68,26 @@ inline cudaError_t launch_pdl(bool early, void (*kernel)(P...), dim3 grid, dim3 
     return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 
+// The same for a kernel whose blocks work in clusters of `cluster` along x.
+template<typename... P, typename... A>
+inline cudaError_t launch_pdl_cluster(bool early, int cluster, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const A &...args)
+{
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = unsigned(cluster);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = early ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
 // Blocks of a plain kernel (threads each) that are all resident at once as far as threads go; where registers or shared memory allow fewer
 // (global pooling's tiles, the banded depthwise kernel) it is a round or two more.  Captured chains of one layer, never early -> early
 // (us): depthwise 3x3 144x56x56 at 1, 4 and 8 images 4.0 -> 3.6, 5.9 -> 5.5, 9.1 -> 8.7, 960x7x7 at 32 8.2 -> 7.9; beyond the line no

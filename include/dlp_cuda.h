@@ -3,10 +3,10 @@
  *
  * This is the whole boundary between host code and CUDA: plain C, plain
  * pointers and sizes, no C++ or framework types.  All pointers named x, w,
- * bias, y, ws, a, b, c are DEVICE pointers to dense fp32 data; every call
- * enqueues work on the CUDA stream it is given (passed as void* = cudaStream_t)
- * and returns without synchronising.  Nothing is allocated inside an enqueue
- * call unless its comment says otherwise; scratch memory is sized by the
+ * bias, y, ws, a, b, c are DEVICE pointers to dense fp32 data (but for the
+ * typed operators at the end, which say what theirs are); every call enqueues
+ * work on the CUDA stream it is given (passed as void* = cudaStream_t) and
+ * returns without synchronising.  Nothing is allocated inside an enqueue call unless its comment says otherwise; scratch memory is sized by the
  * *_workspace() queries and supplied by the caller.
  *
  * Each entry point names the interface of the reference library
@@ -266,6 +266,61 @@ DLP_API dlp_status dlp_softmax_fwd(const float *x, float *y, int rows, int class
 DLP_API dlp_status dlp_batchnorm_inference_fwd(const float *x, float *y, int batch, int features, int plane, float eps,
                                                const float *mean, const float *var, const float *gamma, const float *beta,
                                                void *stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * From a hidden state to a token: the operators around 8-bit products (no counterpart in the reference, whose data is fp32; they stand
+ * beside InnerProduct, BatchNorm, Activation and Softmax above).  Forward only.
+ *
+ * Matrices are row-major with unit stride along a row; strides are in elements and may be anything that keeps rows apart.  Tensors of a
+ * call may not overlap, unless its comment says so.  Elements past a row's end (padding up to its stride) and rows past the last one
+ * are neither read nor written.
+ *
+ * The 8-bit form of a matrix: e4m3 numbers and an fp32 scale for each block, value = number * scale, with
+ * scale = max(largest magnitude / 448, 2^-126) and number = value / scale rounded to the nearest (ties to even).  A block with a NaN or
+ * an infinity has a scale that is NaN or infinite, so that what is computed from it is not finite either.  Blocks are
+ *   - 128 consecutive columns of one row (left operands): scale of block b of row r at scales[b * scale_stride + r], scale_stride >= rows;
+ *   - 128 x 128 (weights): scale of row block i, column block b at scales[i * scale_stride + b], scale_stride >= number of column blocks.
+ * The last block of a row, or of the rows, may be short.  An 8-bit matrix that is an operand of dlp_scaled_ip_fwd has rows on 16-byte
+ * boundaries.
+ * ---------------------------------------------------------------------------------------------- */
+enum { DLP_TYPE_F32 = 0, DLP_TYPE_F16 = 1, DLP_TYPE_BF16 = 2, DLP_TYPE_E4M3 = 3 };
+enum { DLP_GATE_NONE = 0, DLP_GATE_SILU = 1, DLP_GATE_GELU = 2 };
+
+/* Root-mean-square norm of each row, with a residual added before it:
+ *     h = x + residual;   total = h;   y = h / sqrt(mean(h^2) + eps) * weight.
+ * x, residual, total and weight are of `type` (fp32, fp16 or bf16), y of y_type: any of these, or e4m3 in blocks of one row, then with
+ * scales.  h is fp32 throughout; only what is stored is rounded.  residual may be NULL; total may be NULL, or be x or residual itself
+ * (the same address and stride). */
+DLP_API dlp_status dlp_rms_norm_fwd(const void *x, long long x_stride, const void *residual, long long residual_stride, void *total,
+                                    long long total_stride, const void *weight, int type, void *y, long long y_stride, int y_type,
+                                    float *scales, long long scale_stride, int rows, int cols, float eps, void *stream);
+
+/* 8-bit form of x [rows, cols] (gate DLP_GATE_NONE), or of act(a) * b where x [rows, 2 * cols] holds a in its first cols columns and b in the
+ * others: silu(a) = a / (1 + exp(-a)), gelu(a) = a / 2 * (1 + tanh(sqrt(2 / pi) * (a + 0.044715 a^3))), in fp32.  block_rows: 1, or 128 for
+ * weights (without a gate). */
+DLP_API dlp_status dlp_quantize_fwd(const void *x, long long x_stride, int type, int gate, void *q, long long q_stride, float *scales,
+                                    long long scale_stride, int block_rows, int rows, int cols, void *stream);
+
+/* InnerProduct of 8-bit operands, on the tensor cores:
+ *     y[rows, outputs] = act(x[rows, inputs] * w[outputs, inputs]^T + bias[outputs])
+ * x in blocks of one row, w in blocks of 128 x 128.  Products are summed in fp32; y is of y_type (fp32, fp16 or bf16), bias is fp32 or NULL.
+ * x and w are 16-byte aligned, their row strides multiples of 16.  The result does not depend on timing. */
+DLP_API dlp_status dlp_scaled_ip_fwd(const void *x, long long x_stride, const float *x_scales, long long x_scale_stride, const void *w,
+                                     long long w_stride, const float *w_scales, long long w_scale_stride, const float *bias, void *y,
+                                     long long y_stride, int y_type, int activation, int rows, int inputs, int outputs, void *stream);
+
+/* Draws a class from each row of logits (fp32, fp16 or bf16) with the row's random number u, 0 <= u < 1.
+ * With a row's classes in the order of falling logits, equal ones in the order of their index, and masses exp((logit - largest) / temperature):
+ * top_k keeps the first k; top_p keeps of these the shortest prefix that has at least p of their mass (never less than one); min_p keeps of
+ * these the ones whose mass is at least m times the largest one's.  The class drawn is the first one, by index, at which the running mass of
+ * the kept ones exceeds u times their whole mass.
+ * temperature, top_k, top_p, min_p: one value for each row, or NULL (1, and all kept).  A temperature that is not positive means the largest
+ * logit, the lowest index of equal ones; k <= 0 or >= classes, p >= 1 and m <= 0 keep everything; m above 1 counts as 1.  A logit of -inf or
+ * NaN is never drawn; a row of nothing else gives -1.  Logits of +inf share the whole mass.  Masses are summed as whole numbers of at least 41
+ * bits, so the result depends neither on timing nor on the order of sums. */
+#define DLP_SAMPLE_MAX_CLASSES (1 << 22)
+DLP_API dlp_status dlp_sample_fwd(const void *logits, long long stride, int type, int rows, int classes, const float *temperature, const int *top_k,
+                                  const float *top_p, const float *min_p, const float *u, int *tokens, void *stream);
 
 #ifdef __cplusplus
 }
