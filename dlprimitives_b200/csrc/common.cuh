@@ -4,6 +4,8 @@
 #include <stdint.h>
 #include <string>
 #include <atomic>
+#include <mutex>
+#include <vector>
 
 #include "../../include/dlp_cuda.h"
 
@@ -86,6 +88,22 @@ inline cudaError_t launch_pdl_cluster(bool early, int cluster, void (*kernel)(P.
     cfg.attrs = attr;
     cfg.numAttrs = early ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
+// Lets the kernel have this much dynamic shared memory, once per device: the attribute belongs to the function in that device's context.
+template<auto Kernel> inline dlp_status allow_shared(int bytes)
+{
+    static std::mutex mutex;
+    static std::vector<char> configured;          // by device ordinal
+    int dev = 0;
+    DLP_CUDA_OK(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lock(mutex);
+    if(size_t(dev) >= configured.size()) configured.resize(size_t(dev) + 1, 0);
+    if(!configured[dev]) {
+        DLP_CUDA_OK(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        configured[dev] = 1;
+    }
+    return DLP_OK;
 }
 
 // Blocks of a plain kernel (threads each) that are all resident at once as far as threads go; where registers or shared memory allow fewer

@@ -6,7 +6,17 @@
 //
 // Which class it is hangs on sums of up to a few hundred thousand masses, compared with a border.  Masses are whole numbers here,
 // round(w 2^b) with 63 - log2(classes) bits: their sums are exact in any order, so the result depends neither on timing nor on how
-// a row is shared out.  Nothing is sorted: a radix selection on the logits' bits finds where each prefix ends, eight bits a step.
+// a row is shared out.
+//
+// A row is read a few times, from memory once and then from L2, by a cluster of 1 to 8 blocks (so that few rows use the whole GPU); the
+// blocks gather what each has found through distributed shared memory and all come to the same conclusions.
+//   * First the largest logit, and the largest of each of 1024 groups of classes.
+//   * With a small k (up to 512): the k-th largest of the groups' maxima has at least k classes at or above it, in any order of the
+//     classes only a few more (1024 ln(1024 / (1024 - k)) of them are expected).  These are collected, sorted, and the rest is done on
+//     them alone: two readings of the row, and masses of a few hundred classes.
+//   * Otherwise the end of a prefix is found from sums over 2048 bins of falling logits: the bin it lies in is collected and sorted,
+//     and divided further as long as it holds more than 1024 classes.  Then the masses of the kept classes are summed by
+//     segments of the row, and the one segment that the random number points into is gone through.
 #include "block8.cuh"
 
 namespace dlp {
@@ -23,8 +33,11 @@ struct SampleArgs {
     int classes, bits;      // bits of a mass of 1
 };
 
-constexpr int THREADS = 1024, WARPS = THREADS / 32;
+constexpr int THREADS = 1024, WARPS = THREADS / 32, MAX_PARTS = 8;
+constexpr int BINS = 2048, CAP = THREADS;        // bins of a histogram; classes that are sorted at once
+constexpr int SMALL_K = 512;
 constexpr unsigned MASKED = 0;                   // the key of -inf and of NaN
+constexpr unsigned LOWEST = 0x00800000u;         // the key of the lowest finite number
 
 // Keys are ordered as the logits; 0 for classes that cannot be drawn.
 __device__ __forceinline__ unsigned key_of(float v)
@@ -35,184 +48,474 @@ __device__ __forceinline__ unsigned key_of(float v)
 }
 __device__ __forceinline__ float value_of(unsigned key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 
-struct Row {
-    double top, inverse_t, one;                  // largest logit; 1 / temperature; mass of 1
+struct Scratch {
+    u64 mass[BINS], all_mass[BINS];              // of this block's classes; of the row's
+    unsigned count[BINS], all_count[BINS];
+    u64 cand[CAP], sorted[CAP];                  // classes as (key, ~index)
+    u64 seg_mass[WARPS];                         // kept masses of each warp's segment, and classes equal to the cut's key
+    unsigned seg_ties[WARPS];
+    u64 best[WARPS];
+    unsigned group[THREADS];
+    u64 warp_sum[WARPS];
+    u64 found[3];
+    double table[64];                            // 2^(-j / 64)
+    u64 row_best;
+    unsigned cands;
+};
+
+// ---- distributed shared memory: the same place in another block of the cluster
+__device__ __forceinline__ uint32_t place_in(const void *p, int rank)
+{
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ u64 peer(const u64 *p, int rank)
+{
+    u64 v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(place_in(p, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ unsigned peer(const unsigned *p, int rank)
+{
+    unsigned v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(place_in(p, rank)) : "memory");
+    return v;
+}
+
+// A mass of a class.  w = 2^-t with t = (max - x) log2(e) / temperature, in 64 bits: t = i + j / 64 + r with whole i and j, |r| <= 1/128, and
+// 2^-r by the series of exp(-r ln 2), whose sixth term is under 2^-53.
+struct Masses {
+    double top, factor, one, least;              // factor: log2(e) / temperature; one: 2^bits; least: w of min-p
     unsigned top_key;
+    const double *table;
     __device__ __forceinline__ double weight(unsigned key) const
     {
-        return key == top_key ? 1.0 : (key == MASKED ? 0.0 : exp((double(value_of(key)) - top) * inverse_t));
+        if(key == top_key) return 1.0;
+        const double t = (top - double(value_of(key))) * factor;
+        if(!(t < 1000.0)) return 0.0;            // (and an infinite logit's NaN)
+        const double magic = 6755399441055744.0 / 64.0, z = t + magic, r = t - (z - magic);
+        const int k = __double2loint(z);         // 64 i + j
+        constexpr double L = 0.69314718055994530942, C2 = L * L / 2, C3 = L * C2 / 3, C4 = L * C3 / 4, C5 = L * C4 / 5;
+        const double e = fma(r, fma(r, fma(r, fma(r, fma(r, -C5, C4), -C3), C2), -L), 1.0) * table[k & 63];
+        const int i = k >> 6;
+        return __hiloint2double(__double2hiint(e) - (i << 20), __double2loint(e));      // e is in (0.49, 1.01), i under 1001: the exponent stays normal
     }
-    __device__ __forceinline__ u64 mass(unsigned key) const { return u64(__double2ll_rn(weight(key) * one)); }
+    // a whole number below 2^52 is the low part of itself + 2^52
+    __device__ __forceinline__ u64 whole(double w) const { return u64(__double_as_longlong(fma(w, one, 4503599627370496.0)) & 0xfffffffffffffll); }
+    __device__ __forceinline__ u64 mass(unsigned key) const { return key == MASKED ? 0 : whole(weight(key)); }
 };
 
 // Where a prefix of the sorted row ends: all above `key` and the first `ties` of those equal to it.
-struct Cut { unsigned key; unsigned ties; };
+struct Cut { unsigned key, ties; };
 
-struct Shared {
-    u64 mass[256];
-    unsigned count[256];
-    u64 warp_mass[WARPS];
-    unsigned warp_count[WARPS], digit, rest;
-    u64 above;
-    int token;
-};
+// ---- over the block (every thread takes part)
+__device__ __forceinline__ u64 block_scan(u64 v, Scratch &sh, u64 &all)     // sum up to and with this thread's
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    #pragma unroll
+    for(int o = 1; o < 32; o <<= 1) {
+        const u64 other = __shfl_up_sync(0xffffffffu, v, o);
+        if(lane >= o) v += other;
+    }
+    __syncthreads();
+    if(lane == 31) sh.warp_sum[warp] = v;
+    __syncthreads();
+    u64 sums = sh.warp_sum[lane];
+    #pragma unroll
+    for(int o = 1; o < 32; o <<= 1) {
+        const u64 other = __shfl_up_sync(0xffffffffu, sums, o);
+        if(lane >= o) sums += other;
+    }
+    all = __shfl_sync(0xffffffffu, sums, 31);
+    const u64 before = __shfl_sync(0xffffffffu, sums, warp > 0 ? warp - 1 : 0);
+    return v + (warp > 0 ? before : 0);
+}
+// Sorts the threads' numbers, the largest first; `size` (a power of two): threads from there on hold zeros.
+__device__ __forceinline__ u64 block_sort(u64 v, int size, Scratch &sh)
+{
+    const int tid = threadIdx.x;
+    for(int k = 2; k <= size; k <<= 1)
+        for(int j = k >> 1; j > 0; j >>= 1) {
+            u64 other;
+            if(j >= 32) {
+                __syncthreads();
+                sh.sorted[tid] = v;
+                __syncthreads();
+                other = sh.sorted[tid ^ j];
+            }
+            else other = __shfl_xor_sync(0xffffffffu, v, j);
+            const bool larger = ((tid & j) == 0) == ((tid & k) == 0 || k == size);
+            v = larger ? (v > other ? v : other) : (v < other ? v : other);
+        }
+    return v;
+}
 
 template<typename T>
-__global__ void __launch_bounds__(THREADS) sample_kernel(const SampleArgs a)
+__global__ void __launch_bounds__(THREADS, 1) sample_kernel(const SampleArgs a)
 {
     pdl_wait();
-    __shared__ Shared sh;
+    extern __shared__ __align__(16) unsigned char smem[];
+    Scratch &sh = *reinterpret_cast<Scratch *>(smem);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.classes;
-    const long long row = blockIdx.x;
+    int parts, part;
+    asm volatile("mov.u32 %0, %cluster_nctarank;" : "=r"(parts));
+    asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(part));
+    const long long row = blockIdx.x / parts;
     const T *x = static_cast<const T *>(a.x) + row * a.stride;
-    auto key_at = [&](int i) { return key_of(to_float(ld_plain(x + i))); };
+    auto everyone = [&] {
+        if(parts > 1) {
+            asm volatile("barrier.cluster.arrive;" ::: "memory");
+            asm volatile("barrier.cluster.wait;" ::: "memory");
+        }
+        else __syncthreads();
+    };
 
-    unsigned top = MASKED;
-    for(int i = tid; i < n; i += THREADS) top = max(top, key_at(i));
-    top = __reduce_max_sync(0xffffffffu, top);
-    if(lane == 0) sh.warp_count[warp] = top;
-    __syncthreads();
-    for(int i = 0; i < WARPS; i++) top = max(top, sh.warp_count[i]);
-    if(top == MASKED) {                          // nothing to draw from
-        if(tid == 0) a.tokens[row] = -1;
-        return;
+    // The row in pieces of 16 bytes on their boundaries; each warp of the cluster has a segment of consecutive ones.
+    constexpr int V = 16 / sizeof(T);
+    const int shift = int(reinterpret_cast<uintptr_t>(x) / sizeof(T) % V);
+    const int pieces = (n + shift + V - 1) / V, per = ceil_div(pieces, parts * WARPS);
+    const int piece0 = (part * WARPS + warp) * per, piece1 = min(pieces, piece0 + per);
+    // f(key, index) for the segment's classes; a thread's come in index order
+    auto each = [&](auto f) {
+        constexpr int DEEP = 4;
+        for(int p = piece0 + lane; p < piece1; p += 32 * DEEP) {
+            union { uint4 w; T e[V]; } u[DEEP];
+            #pragma unroll
+            for(int d = 0; d < DEEP; d++) {
+                const int i0 = (p + d * 32) * V - shift;
+                if(p + d * 32 < piece1 && i0 >= 0 && i0 + V <= n) u[d].w = ld_plain(reinterpret_cast<const uint4 *>(x + i0));
+            }
+            #pragma unroll
+            for(int d = 0; d < DEEP; d++) {
+                const int i0 = (p + d * 32) * V - shift;
+                if(p + d * 32 >= piece1) break;
+                if(i0 >= 0 && i0 + V <= n) {
+                    #pragma unroll
+                    for(int e = 0; e < V; e++) f(key_of(to_float(u[d].e[e])), i0 + e);
+                }
+                else
+                    for(int e = 0; e < V; e++)
+                        if(i0 + e >= 0 && i0 + e < n) f(key_of(to_float(ld_plain(x + i0 + e))), i0 + e);
+            }
+        }
+    };
+
+    // ---- the largest logit, its first place, and the groups' largest (a group: `parts` neighbouring threads)
+    if(tid < 64) sh.table[tid] = exp2(tid * (-1.0 / 64));
+    unsigned most = MASKED;
+    int where = 0;
+    each([&](unsigned key, int i) {
+        if(key > most) { most = key; where = i; }
+    });
+    u64 best = u64(most) << 32 | unsigned(~where);
+    unsigned group = most;
+    for(int o = 1; o < parts; o <<= 1) group = max(group, __shfl_xor_sync(0xffffffffu, group, o));
+    if(tid % parts == 0) sh.group[tid / parts] = group;
+    #pragma unroll
+    for(int o = 16; o > 0; o >>= 1) {
+        const u64 other = __shfl_xor_sync(0xffffffffu, best, o);
+        best = other > best ? other : best;
+    }
+    if(lane == 0) sh.best[warp] = best;
+    if(tid == 0) sh.cands = 0;
+    everyone();
+    {
+        const int per_part = THREADS / parts;
+        group = parts > 1 ? peer(sh.group + tid % per_part, tid / per_part) : sh.group[tid];
+    }
+    for(int i = lane; i < parts * WARPS; i += 32) {
+        const u64 other = parts > 1 ? peer(sh.best + i % WARPS, i / WARPS) : sh.best[i];
+        best = other > best ? other : best;
+    }
+    #pragma unroll
+    for(int o = 16; o > 0; o >>= 1) {
+        const u64 other = __shfl_xor_sync(0xffffffffu, best, o);
+        best = other > best ? other : best;
     }
     const float t = a.temperature ? ld_plain(a.temperature + row) : 1.0f;
     const bool greedy = !(t > 0.0f);
-    Row r;
-    r.top_key = top;
-    r.top = double(value_of(top));
-    r.inverse_t = greedy ? 1.0 : 1.0 / double(t);
-    r.one = double(1ull << a.bits);
     const int k = greedy ? 1 : (a.top_k ? ld_plain(a.top_k + row) : 0);
     const float p = a.top_p ? ld_plain(a.top_p + row) : 1.0f, m = a.min_p ? ld_plain(a.min_p + row) : 0.0f, uf = ld_plain(a.u + row);
+    const unsigned top = unsigned(best >> 32);
+    if(top == MASKED || k == 1) {                // nothing to draw from, or one
+        if(part == 0 && tid == 0) a.tokens[row] = top == MASKED ? -1 : int(~unsigned(best));
+        everyone();                              // nobody leaves while its memory is being read
+        return;
+    }
+    Masses f;
+    f.top_key = top;
+    f.top = double(value_of(top));
+    f.factor = 1.4426950408889634074 / double(t);
+    f.one = double(1ull << a.bits);
+    f.least = m > 0.0f ? fmin(double(m), 1.0) : 0.0;
+    f.table = sh.table;
+    // the least whole number that is no less than p times `whole`
+    auto share_of = [&](u64 whole) {
+        const u64 pf = p > 0.0f ? u64(double(p) * 18446744073709551616.0) : 0;
+        const u64 want = __umul64hi(pf, whole) + (pf * whole != 0);
+        return want > 0 ? want : 1;
+    };
+    auto point_in = [&](u64 whole) { return __umul64hi(uf > 0.0f ? (uf < 1.0f ? u64(double(uf) * 18446744073709551616.0) : ~0ull) : 0ull, whole); };
 
-    // The end of the shortest prefix that holds `want` classes, or that much mass, of the classes that `limit` keeps; the mass above its key.
-    auto select = [&](bool by_mass, u64 want, Cut limit, u64 &above) {
-        unsigned prefix = 0;
-        above = 0;
-        u64 left = want;
-        unsigned equal = 0;
-        for(int shift = 24; shift >= 0; shift -= 8) {
-            __syncthreads();
-            if(tid < 256) { sh.mass[tid] = 0; sh.count[tid] = 0; }
-            __syncthreads();
-            for(int i = tid; i < n; i += THREADS) {
-                const unsigned key = key_at(i);
-                if(key == MASKED || key < limit.key || (shift < 24 && (key ^ prefix) >> (shift + 8))) continue;
-                const unsigned d = key >> shift & 255;
-                atomicAdd(&sh.mass[d], r.mass(key));
-                atomicAdd(&sh.count[d], 1u);
+    // Collects the classes with lo <= key <= hi in every block's list (all of the row's).  Their number; the list holds them if that is at most CAP.
+    auto collect = [&](unsigned lo, unsigned hi) {
+        each([&](unsigned key, int i) {
+            if(key >= lo && key <= hi) {
+                const unsigned at = atomicAdd(&sh.cands, 1u);
+                if(at < CAP) sh.cand[at] = u64(key) << 32 | unsigned(~i);
             }
-            __syncthreads();
-            if(tid == 0) {
-                u64 more = 0;
-                int d = 255;
-                for(; d > 0; d--) {
-                    u64 here = by_mass ? sh.mass[d] : sh.count[d];
-                    // (of the limit's own key only the first ties count)
-                    if(by_mass && shift == 0 && (prefix | d) == limit.key && limit.ties < sh.count[d]) here = limit.ties * r.mass(limit.key);
-                    if(here >= left) break;
-                    left -= here;
-                    more += sh.mass[d];
-                }
-                sh.digit = d;
-                sh.above = more;
-                sh.rest = sh.count[d];
-                sh.mass[0] = left;
-            }
-            __syncthreads();
-            prefix |= sh.digit << shift;
-            above += sh.above;
-            left = sh.mass[0];
-            equal = sh.rest;
+        });
+        everyone();
+        unsigned total = 0;
+        int from = 0;
+        unsigned place = 0;
+        for(int q = 0; q < parts; q++) {
+            const unsigned c = parts > 1 ? peer(&sh.cands, q) : sh.cands;
+            if(unsigned(tid) >= total && unsigned(tid) < total + c) { from = q; place = tid - total; }
+            total += c;
         }
+        u64 mine = 0;
+        if(total <= CAP && unsigned(tid) < total) mine = parts > 1 ? peer(sh.cand + place, from) : sh.cand[place];
+        everyone();
+        if(tid == 0) sh.cands = 0;
+        int size = 32;
+        while(size < int(total) && size < CAP) size <<= 1;
+        const u64 sorted = total <= CAP ? block_sort(mine, size, sh) : 0;
+        __syncthreads();
+        return make_ulonglong2(total, sorted);
+    };
+
+    // ---- few classes are kept: all of them in one sorted list
+    const bool few = k > 0 && k <= SMALL_K && k < n;
+    if(few || n <= CAP) {
+        unsigned floor_key = 1;
+        if(few) {
+            // the k-th largest of the groups' maxima, from the top bit down (but for the last eight: a little lower is as good)
+            unsigned at = 0;
+            for(int bit = 31; bit >= 8; bit--) {
+                const unsigned higher = at | 1u << bit;
+                if(__syncthreads_count(group >= higher) >= k) at = higher;
+            }
+            floor_key = max(at, 1u);
+        }
+        const ulonglong2 got = collect(floor_key, 0xffffffffu);
+        const int total = int(got.x);
+        if(got.x <= CAP) {
+            const unsigned key = unsigned(got.y >> 32);
+            const int kept_k = k > 0 && k < total ? k : total;
+            const double w = tid < kept_k ? f.weight(key) : 0.0;
+            u64 mass = tid < kept_k ? f.whole(w) : 0, whole, run = block_scan(mass, sh, whole);
+            if(!greedy && p < 1.0f && run - mass >= share_of(whole)) mass = 0;
+            if(w < f.least) mass = 0;
+            // in index order: by ~index, the largest first, with the place of the mass
+            __syncthreads();
+            sh.mass[tid] = mass;
+            int size = 32;
+            while(size < kept_k) size <<= 1;
+            const u64 by_index = block_sort(mass ? (got.y & 0xffffffffull) << 32 | unsigned(tid) : 0, size, sh);
+            __syncthreads();
+            mass = by_index ? sh.mass[unsigned(by_index)] : 0;
+            run = block_scan(mass, sh, whole);
+            const u64 target = point_in(whole);
+            if(part == 0 && mass && run > target && run - mass <= target) a.tokens[row] = int(~unsigned(by_index >> 32));
+            return;                              // (the lists were gathered between two barriers: nobody reads another's memory any more)
+        }
+    }
+
+    // ---- the ends of long prefixes
+    const float bin_scale = fminf(float(BINS) / (30.0f * t), 1e30f), top_value = value_of(top);
+    // bin of a key, 0 for the largest logits
+    auto bin_of = [&](unsigned key) { return key == top ? 0 : int(fminf((top_value - value_of(key)) * bin_scale, float(BINS - 1))); };
+    // Sums over bins of the classes with lo <= key <= hi, the same in every block; shift < 0: bins of logits, else of (hi - key) >> shift
+    auto histogram = [&](unsigned lo, unsigned hi, int bits) {
+        __syncthreads();
+        for(int i = tid; i < BINS; i += THREADS) { sh.mass[i] = 0; sh.count[i] = 0; }
+        __syncthreads();
+        each([&](unsigned key, int) {
+            if(key < lo || key > hi || key == MASKED) return;
+            const int b = bits < 0 ? bin_of(key) : int((hi - key) >> bits);
+            atomicAdd(&sh.mass[b], f.mass(key));
+            atomicAdd(&sh.count[b], 1u);
+        });
+        everyone();
+        for(int i = tid; i < BINS; i += THREADS) {
+            u64 s = 0;
+            unsigned c = 0;
+            for(int q = 0; q < parts; q++) {
+                s += parts > 1 ? peer(sh.mass + i, q) : sh.mass[i];
+                c += parts > 1 ? peer(sh.count + i, q) : sh.count[i];
+            }
+            sh.all_mass[i] = s;
+            sh.all_count[i] = c;
+        }
+        everyone();
+    };
+    // The bin in which the running sum (of masses, or of numbers) reaches `want`: it, and the sums before it.
+    auto find_bin = [&](bool by_mass, u64 want, u64 &mass_before, u64 &count_before) {
+        const u64 m0 = sh.all_mass[2 * tid], m1 = sh.all_mass[2 * tid + 1];
+        const u64 c0 = sh.all_count[2 * tid], c1 = sh.all_count[2 * tid + 1];
+        u64 whole;
+        const u64 ms = block_scan(m0 + m1, sh, whole) - m0 - m1, cs = block_scan(c0 + c1, sh, whole) - c0 - c1;
+        const u64 s = by_mass ? ms : cs, v0 = by_mass ? m0 : c0, v1 = by_mass ? m1 : c1;
+        if(s < want && s + v0 >= want) { sh.found[0] = 2 * tid; sh.found[1] = ms; sh.found[2] = cs; }
+        else if(s + v0 < want && s + v0 + v1 >= want) { sh.found[0] = 2 * tid + 1; sh.found[1] = ms + m0; sh.found[2] = cs + c0; }
+        __syncthreads();
+        mass_before = sh.found[1];
+        count_before = sh.found[2];
+        return int(sh.found[0]);
+    };
+    // The end of the shortest prefix with `want` classes, or that much mass, and its mass.  The sums over the bins of all logits are in place.
+    auto find_cut = [&](bool by_mass, u64 want, u64 &mass) {
         Cut c;
-        c.key = prefix;
-        const u64 w = r.mass(prefix);
-        const u64 need = by_mass ? (w ? (left + w - 1) / w : 1) : left;
-        c.ties = unsigned(need < equal ? need : equal);
-        if(c.key == limit.key && c.ties > limit.ties) c.ties = limit.ties;
+        u64 mass_before, count_before;
+        int b = find_bin(by_mass, want, mass_before, count_before);
+        // the keys of that bin
+        unsigned lo = LOWEST, hi = top;
+        {
+            unsigned l = LOWEST - 1, h = top;                // the least key with bin <= b
+            while(h - l > 1) { const unsigned mid = l + (h - l) / 2; if(bin_of(mid) <= b) h = mid; else l = mid; }
+            lo = h;
+            if(b > 0) {
+                l = lo - 1; h = top;                         // the least key with bin < b, less one
+                while(h - l > 1) { const unsigned mid = l + (h - l) / 2; if(bin_of(mid) < b) h = mid; else l = mid; }
+                hi = h - 1;
+            }
+        }
+        mass = mass_before;
+        u64 left = want - (by_mass ? mass_before : count_before);
+        unsigned equal = sh.all_count[b];
+        while(equal > CAP && lo < hi) {
+            int bits = 0;
+            while((hi - lo) >> bits >= BINS) bits++;
+            histogram(lo, hi, bits);
+            b = find_bin(by_mass, left, mass_before, count_before);
+            mass += mass_before;
+            left -= by_mass ? mass_before : count_before;
+            equal = sh.all_count[b];
+            const unsigned from = hi - (unsigned(b) << bits);
+            lo = max(lo, from - ((1u << bits) - 1));
+            hi = from;
+        }
+        if(equal > CAP) {                                    // more equal logits than are sorted at once
+            const u64 w = f.mass(hi), need = by_mass ? (left + w - 1) / w : left;
+            c.key = hi;
+            c.ties = unsigned(need);
+            mass += need * w;
+            return c;
+        }
+        const ulonglong2 got = collect(lo, hi);
+        const unsigned key = unsigned(got.y >> 32);
+        const bool in = unsigned(tid) < got.x;
+        u64 whole;
+        const u64 w = in ? f.mass(key) : 0, run = block_scan(w, sh, whole);
+        const bool last = in && (by_mass ? run >= left && run - w < left : u64(tid) + 1 == left);
+        __syncthreads();
+        sh.sorted[tid] = got.y;
+        if(last) { sh.found[0] = tid; sh.found[1] = run; }
+        __syncthreads();
+        const int at = int(sh.found[0]);
+        mass += sh.found[1];
+        c.key = unsigned(sh.sorted[at] >> 32);
+        c.ties = __syncthreads_count(in && tid <= at && key == c.key);
         return c;
     };
 
-    Cut cut = { 1u, 0xffffffffu };
-    u64 whole = 0;
-    bool known = false;                          // whole: the mass of what `cut` keeps
-    if(k > 0 && k < n) {
-        cut = select(false, u64(k), cut, whole);
-        whole += cut.ties * r.mass(cut.key);
-        known = true;
-    }
-    if(!greedy && p < 1.0f) {
-        if(!known) {
-            u64 mine = 0;
-            for(int i = tid; i < n; i += THREADS) mine += r.mass(key_at(i));
-            for(int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-            __syncthreads();
-            if(lane == 0) sh.warp_mass[warp] = mine;
-            __syncthreads();
-            for(int i = 0; i < WARPS; i++) whole += sh.warp_mass[i];
+    Cut cut = { 0, 0 };
+    const bool by_count = k > 0 && k < n, by_mass = p < 1.0f;
+    if(by_count || by_mass) {
+        histogram(1, 0xffffffffu, -1);
+        u64 whole = 0, at_most;
+        {
+            const u64 mine = sh.all_mass[2 * tid] + sh.all_mass[2 * tid + 1], number = sh.all_count[2 * tid] + sh.all_count[2 * tid + 1];
+            block_scan(mine, sh, whole);
+            block_scan(number, sh, at_most);
         }
-        // the least whole number that is no less than p * whole
-        const u64 pf = p > 0.0f ? u64(double(p) * 18446744073709551616.0) : 0;
-        u64 want = __umul64hi(pf, whole) + (pf * whole != 0);
-        if(want == 0) want = 1;
-        u64 above;
-        cut = select(true, want, cut, above);
+        bool fresh = true;                                   // the sums are those of all logits
+        if(by_count && u64(k) < at_most) {
+            cut = find_cut(false, u64(k), whole);
+            fresh = false;
+        }
+        if(by_mass) {
+            if(!fresh) histogram(1, 0xffffffffu, -1);
+            u64 mass;
+            const Cut shorter = find_cut(true, share_of(whole), mass);
+            cut = shorter;
+        }
     }
 
-    // Masses in index order: the whole of the kept ones first, then where the running sum passes u times that.
-    const double least = m > 0.0f ? fmin(double(m), 1.0) : 0.0;
-    u64 target = 0;
-    for(int pass = 0; pass < 2; pass++) {
-        u64 before = 0;
-        unsigned ties_before = 0;
-        if(pass == 1 && tid == 0) sh.token = n;
-        for(int i0 = 0; i0 < n; i0 += THREADS) {
-            const int i = i0 + tid;
-            const unsigned key = i < n ? key_at(i) : MASKED;
-            const bool tie = key == cut.key;
-            const unsigned votes = __ballot_sync(0xffffffffu, tie);
-            __syncthreads();
-            if(lane == 0) sh.warp_count[warp] = __popc(votes);
-            __syncthreads();
-            unsigned ties = ties_before + __popc(votes & ((1u << lane) - 1));
-            for(int j = 0; j < WARPS; j++) {
-                if(j < warp) ties += sh.warp_count[j];
-                ties_before += sh.warp_count[j];
+    // ---- kept masses by segments
+    {
+        u64 sure = 0;
+        unsigned ties = 0;
+        each([&](unsigned key, int) {
+            if(key == MASKED || key < cut.key) return;
+            if(key == cut.key) ties++;
+            else {
+                const double w = f.weight(key);
+                if(w >= f.least) sure += f.whole(w);
             }
-            u64 w = 0;
-            if(key > cut.key || (tie && ties < cut.ties)) {
-                const double f = r.weight(key);
-                if(f >= least) w = u64(__double2ll_rn(f * r.one));
-            }
-            u64 run = w;
-            for(int o = 1; o < 32; o <<= 1) {
-                const u64 other = __shfl_up_sync(0xffffffffu, run, o);
-                if(lane >= o) run += other;
-            }
-            if(lane == 31) sh.warp_mass[warp] = run;
-            __syncthreads();
-            run += before;
-            for(int j = 0; j < WARPS; j++) {
-                if(j < warp) run += sh.warp_mass[j];
-                before += sh.warp_mass[j];
-            }
-            if(pass == 1 && w > 0 && run > target && run - w <= target) sh.token = i;
-        }
-        if(pass == 0) {
-            const u64 uu = uf > 0.0f ? (uf < 1.0f ? u64(double(uf) * 18446744073709551616.0) : ~0ull) : 0;
-            target = __umul64hi(uu, before);
-        }
+        });
+        #pragma unroll
+        for(int o = 16; o > 0; o >>= 1) sure += __shfl_xor_sync(0xffffffffu, sure, o);
+        ties = __reduce_add_sync(0xffffffffu, ties);
+        if(lane == 0) { sh.seg_mass[warp] = sure; sh.seg_ties[warp] = ties; }
     }
+    everyone();
+    u64 tie_mass = 0;
+    if(cut.key) {
+        const double w = f.weight(cut.key);
+        if(w >= f.least) tie_mass = f.whole(w);
+    }
+    const int segs = parts * WARPS;
+    u64 seg = 0, seg_ties = 0;
+    if(tid < segs) {
+        seg = parts > 1 ? peer(sh.seg_mass + tid % WARPS, tid / WARPS) : sh.seg_mass[tid];
+        seg_ties = parts > 1 ? peer(sh.seg_ties + tid % WARPS, tid / WARPS) : sh.seg_ties[tid];
+    }
+    everyone();
+    u64 whole;
+    const u64 ties_to = block_scan(seg_ties, sh, whole), ties_before = ties_to - seg_ties;
+    if(seg_ties && ties_before < cut.ties) seg += tie_mass * min(seg_ties, cut.ties - ties_before);
+    const u64 run = block_scan(seg, sh, whole), target = point_in(whole);
+    if(seg && run > target && run - seg <= target) { sh.found[0] = tid; sh.found[1] = run - seg; sh.found[2] = ties_before; }
     __syncthreads();
-    if(tid == 0) a.tokens[row] = sh.token;
+    const int seg_at = int(sh.found[0]);
+    u64 before = sh.found[1], ties_seen = sh.found[2];
+    if(seg_at / WARPS != part) return;
+
+    // ---- the segment that the random number points into, a stretch of consecutive classes at a time
+    const int from = max(0, seg_at * per * V - shift), to = int(min((long long)n, (long long)(seg_at + 1) * per * V - shift));
+    for(int i0 = from; i0 < to; i0 += THREADS) {
+        const int i = i0 + tid;
+        const unsigned key = i < to ? key_of(to_float(ld_plain(x + i))) : MASKED;
+        const bool tie = key != MASKED && key == cut.key;
+        u64 all_ties = 0, all;
+        const u64 rank = cut.key ? block_scan(tie ? 1 : 0, sh, all_ties) : 0;
+        u64 mass = 0;
+        if(tie) mass = ties_seen + rank <= cut.ties ? tie_mass : 0;
+        else if(key > cut.key) {
+            const double w = f.weight(key);
+            if(w >= f.least) mass = f.whole(w);
+        }
+        const u64 to_here = before + block_scan(mass, sh, all);
+        if(mass && to_here > target && to_here - mass <= target) a.tokens[row] = i;
+        before += all;
+        ties_seen += all_ties;
+        if(before > target) return;              // (the same in every thread)
+    }
 }
 
 template<typename T> dlp_status launch_sample(const SampleArgs &a, int rows, cudaStream_t stream)
 {
-    DLP_LAUNCH_PDL(launch_pdl(one_wave(rows, THREADS), sample_kernel<T>, rows, THREADS, 0, stream, a), "sample_kernel");
+    const dlp_status st = allow_shared<sample_kernel<T>>(int(sizeof(Scratch)));
+    if(st != DLP_OK) return st;
+    // blocks of a row: as many as there are SMs for, with 8192 classes or more to each
+    int parts = 1;
+    while(parts < MAX_PARTS && (long long)rows * parts * 2 <= sm_count() && a.classes / (parts * 2) >= 8192) parts *= 2;
+    DLP_REQUIRE((long long)rows * parts < (1ll << 31), "too many rows");
+    DLP_LAUNCH_PDL(launch_pdl_cluster(one_wave((long long)rows * parts, THREADS), parts, sample_kernel<T>, rows * parts, THREADS, sizeof(Scratch), stream, a),
+                   "sample_kernel");
     return DLP_OK;
 }
 
@@ -235,7 +538,7 @@ dlp_status dlp_sample_fwd(const void *logits, long long stride, int type, int ro
                 aligned_to(top_p, 4) && aligned_to(min_p, 4), "a tensor is not aligned to its elements");
     int log2 = 0;
     while((1ll << log2) < classes) log2++;
-    const SampleArgs a = { logits, temperature, top_p, min_p, u, top_k, tokens, stride, classes, std::min(52, 63 - log2) };
+    const SampleArgs a = { logits, temperature, top_p, min_p, u, top_k, tokens, stride, classes, std::min(51, 63 - log2) };
     if(type == DLP_TYPE_F32) return launch_sample<float>(a, rows, (cudaStream_t)stream);
     if(type == DLP_TYPE_F16) return launch_sample<__half>(a, rows, (cudaStream_t)stream);
     return launch_sample<__nv_bfloat16>(a, rows, (cudaStream_t)stream);

@@ -13,8 +13,6 @@
 #include "tc_device.cuh"
 #include <cuda.h>
 #include <cstring>
-#include <mutex>
-#include <vector>
 
 namespace dlp {
 namespace sip {
@@ -319,22 +317,12 @@ constexpr int SMEM_LIMIT = 227 * 1024;
 template<int BN, bool SWAP>
 static dlp_status launch(const void *x, long long x_stride, const void *w, long long w_stride, int inputs, Params q, int parts, cudaStream_t stream)
 {
-    {
-        static std::mutex mutex;
-        static std::vector<char> configured;          // by device ordinal: the attribute belongs to the function in that device's context
-        int dev = 0;
-        DLP_CUDA_OK(cudaGetDevice(&dev));
-        std::lock_guard<std::mutex> lock(mutex);
-        if(size_t(dev) >= configured.size()) configured.resize(size_t(dev) + 1, 0);
-        if(!configured[dev]) {
-            DLP_CUDA_OK(cudaFuncSetAttribute(scaled_ip_kernel<BN, SWAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT));
-            configured[dev] = 1;
-        }
-    }
+    dlp_status st = allow_shared<scaled_ip_kernel<BN, SWAP>>(SMEM_LIMIT);
+    if(st != DLP_OK) return st;
     int *status = device_status_word();
     if(!status) return fail(DLP_CUDA_ERROR, "cannot resolve the device status word");
     CUtensorMap mx, mw;
-    dlp_status st = encode(mx, x, x_stride, q.rows, inputs, SWAP ? BN : BM);
+    st = encode(mx, x, x_stride, q.rows, inputs, SWAP ? BN : BM);
     if(st == DLP_OK) st = encode(mw, w, w_stride, q.outputs, inputs, SWAP ? BM : BN);
     if(st != DLP_OK) return st;
     const int fixed = 2048 + 2 * SC_CHUNK * (SWAP ? BN : BM) * 4, stage = (BM + BN) * BK;
