@@ -9,22 +9,16 @@
 //     K is cut into parts over the blocks of a cluster, so that a product of few tiles reads its weights with the whole GPU; the parts are
 //     added through distributed shared memory in a fixed order.
 // Every wait is bounded (device status word + abort flag).
-#include "block8.cuh"
-#include "tc_device.cuh"
-#include <cuda.h>
+#include "scaled_ip.cuh"
 #include <cstring>
 
 namespace dlp {
 namespace sip {
 
-using namespace tc;
-
-constexpr int BM = 128, BK = 128;           // a tile's rows; a block of K, one 128-byte row of the swizzled operand tiles
 constexpr int SC_CHUNK = 16;                // blocks of K whose scales are brought in at a time
 constexpr int MAX_STAGES = 12;
 constexpr int NUM_THREADS = 192;            // copies, MMA issue, four warps that sum and store
 constexpr int MAX_CLUSTER = 8;
-enum { SIP_EMPTY = 501, SIP_FULL = 502, SIP_ACC_EMPTY = 503, SIP_ACC_FULL = 504, SIP_DRAIN = 505 };
 
 struct Shared {
     unsigned long long full[MAX_STAGES], empty[MAX_STAGES], acc_full[4], acc_empty[4], drain;
@@ -59,19 +53,10 @@ template<int BN> __device__ __forceinline__ void mma_block(uint32_t d, uint64_t 
                      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
                      ::"r"(d), "l"(a + 2 * j), "l"(b + 2 * j), "r"(idesc_e4m3(BN)), "r"(j) : "memory");
 }
-__device__ __forceinline__ void cluster_sync()
-{
-    asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm volatile("mov.u32 %0, %cluster_nctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank)
 {
-    uint32_t remote;
     float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(place_in(addr, rank)) : "memory");
     return v;
 }
 
@@ -299,31 +284,42 @@ static EncodeTiledFn encode_fn()
     }
     return fn;
 }
-// an 8-bit matrix in boxes of 128 columns x box_rows rows
-static dlp_status encode(CUtensorMap &map, const void *p, long long stride, int rows, int cols, int box_rows)
+static dlp_status encode_2d(CUtensorMap &map, CUtensorMapDataType type, const void *p, long long cols, long long rows, long long stride_bytes, int box_cols,
+                            int box_rows)
 {
     EncodeTiledFn enc = encode_fn();
     if(!enc) return fail(DLP_CUDA_ERROR, "cuTensorMapEncodeTiled is not available from this driver");
-    cuuint64_t dims[2] = { cuuint64_t(cols), cuuint64_t(rows) }, strides[1] = { cuuint64_t(rows > 1 ? stride : round_up(cols, 16)) };
-    cuuint32_t box[2] = { BK, cuuint32_t(box_rows) }, elem[2] = { 1, 1 };
-    const CUresult r = enc(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(p), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    cuuint64_t dims[2] = { cuuint64_t(cols), cuuint64_t(rows) }, strides[1] = { cuuint64_t(stride_bytes) };
+    cuuint32_t box[2] = { cuuint32_t(box_cols), cuuint32_t(box_rows) }, elem[2] = { 1, 1 };
+    const CUresult r = enc(&map, type, 2, const_cast<void *>(p), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if(r != CUDA_SUCCESS) return fail(DLP_CUDA_ERROR, "cuTensorMapEncodeTiled failed with code " + std::to_string(int(r)));
     return DLP_OK;
 }
-
-constexpr int SMEM_LIMIT = 227 * 1024;
+dlp_status encode_operand(CUtensorMap &map, const void *p, long long stride, int rows, int cols, int box_rows)
+{
+    return encode_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, p, cols, rows, rows > 1 ? stride : round_up(cols, 16), BK, box_rows);
+}
+dlp_status encode_result(CUtensorMap &map, const Problem &p)
+{
+    const int size = type_size(p.y_type);
+    const CUtensorMapDataType type = p.y_type == DLP_TYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                                              : (p.y_type == DLP_TYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
+    return encode_2d(map, type, p.y, p.outputs, p.rows, p.y_stride * size, 128 / size, 32);
+}
 
 template<int BN, bool SWAP>
-static dlp_status launch(const void *x, long long x_stride, const void *w, long long w_stride, int inputs, Params q, int parts, cudaStream_t stream)
+static dlp_status launch(const Problem &p, int parts, cudaStream_t stream)
 {
     dlp_status st = allow_shared<scaled_ip_kernel<BN, SWAP>>(SMEM_LIMIT);
     if(st != DLP_OK) return st;
     int *status = device_status_word();
     if(!status) return fail(DLP_CUDA_ERROR, "cannot resolve the device status word");
+    Params q = { p.x_scales, p.w_scales, p.bias, p.y, p.x_scale_stride, p.w_scale_stride, p.y_stride, p.rows, p.outputs, p.kblocks,
+                 ceil_div(p.kblocks, parts), 0, p.y_type, p.act, 0 };
     CUtensorMap mx, mw;
-    st = encode(mx, x, x_stride, q.rows, inputs, SWAP ? BN : BM);
-    if(st == DLP_OK) st = encode(mw, w, w_stride, q.outputs, inputs, SWAP ? BM : BN);
+    st = encode_operand(mx, p.x, p.x_stride, p.rows, p.inputs, SWAP ? BN : BM);
+    if(st == DLP_OK) st = encode_operand(mw, p.w, p.w_stride, p.outputs, p.inputs, SWAP ? BM : BN);
     if(st != DLP_OK) return st;
     const int fixed = 2048 + 2 * SC_CHUNK * (SWAP ? BN : BM) * 4, stage = (BM + BN) * BK;
     q.stages = std::min(MAX_STAGES, (SMEM_LIMIT - fixed) / stage);
@@ -361,29 +357,17 @@ dlp_status dlp_scaled_ip_fwd(const void *x, long long x_stride, const float *x_s
     DLP_REQUIRE((rows <= 1 || x_stride < (1ll << 40)) && (outputs == 1 || w_stride < (1ll << 40)), "a row stride must be under 2^40");
     DLP_REQUIRE(aligned_to(x_scales, 4) && aligned_to(w_scales, 4) && (!bias || aligned_to(bias, 4)) && aligned_to(y, type_size(y_type)),
                 "a tensor is not aligned to its elements");
-    sip::Params q = {};
-    q.x_scales = x_scales;
-    q.w_scales = w_scales;
-    q.bias = bias;
-    q.y = y;
-    q.x_scale_stride = x_scale_stride;
-    q.w_scale_stride = w_scale_stride;
-    q.y_stride = y_stride;
-    q.rows = rows;
-    q.outputs = outputs;
-    q.kblocks = q.per_part = kblocks;
-    q.y_type = y_type;
-    q.act = activation;
+    const sip::Problem p = { x, w, x_stride, w_stride, x_scales, w_scales, bias, y, x_scale_stride, w_scale_stride, y_stride, rows, inputs, outputs,
+                             kblocks, y_type, activation };
     cudaStream_t s = (cudaStream_t)stream;
-    if(rows > 128) return sip::launch<128, false>(x, x_stride, w, w_stride, inputs, q, 1, s);
+    if(rows > 128) return sip::launch_pair(p, s);
     // parts of K until every SM has a tile
     int parts = 1;
     while(parts < sip::MAX_CLUSTER && parts * 2 <= kblocks && oblocks * parts * 2 <= sm_count()) parts *= 2;
-    q.per_part = ceil_div(kblocks, parts);
-    if(rows <= 16) return sip::launch<16, true>(x, x_stride, w, w_stride, inputs, q, parts, s);
-    if(rows <= 32) return sip::launch<32, true>(x, x_stride, w, w_stride, inputs, q, parts, s);
-    if(rows <= 64) return sip::launch<64, true>(x, x_stride, w, w_stride, inputs, q, parts, s);
-    return sip::launch<128, true>(x, x_stride, w, w_stride, inputs, q, parts, s);
+    if(rows <= 16) return sip::launch<16, true>(p, parts, s);
+    if(rows <= 32) return sip::launch<32, true>(p, parts, s);
+    if(rows <= 64) return sip::launch<64, true>(p, parts, s);
+    return sip::launch<128, true>(p, parts, s);
 }
 
 } // extern "C"
