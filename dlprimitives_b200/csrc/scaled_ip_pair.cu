@@ -7,12 +7,13 @@
 // pair reads a row of w once where two single SMs would read it twice.
 //   * one warp per SM issues the tensor-map copies of its half; both halves' bytes are counted on the leader's barrier;
 //   * one thread of the leader issues the MMAs of the pair; its commits go to both SMs;
-//   * eight warps per SM sum: a quarter of the rows and half of the columns each.  They bring the scales in by 4-byte asynchronous copies,
-//     eight blocks ahead, each thread its own (no barrier), and store through shared memory and tensor-map stores.
+//   * eight warps per SM sum: a quarter of the rows and half of the columns each.  Each thread loads its scales
+//     three blocks ahead.  They store through shared memory and tensor-map stores.
 // Tiles are taken in turn (persistent blocks), eight row tiles at a time down the columns, so that what the SMs read at one time stays in L2.
 // Every wait is bounded.
 #define DLP_INLINE_WAITS
 #include "scaled_ip.cuh"
+#include <algorithm>
 
 namespace dlp {
 namespace sip {
@@ -23,7 +24,7 @@ constexpr int NUM_THREADS = 384, SUM_WARPS = 8;
 constexpr int REGS_LAUNCH = 168, REGS_ISSUE = 40, REGS_SUM = 232;
 static_assert(REGS_ISSUE + 2 * REGS_SUM <= 3 * REGS_LAUNCH, "setmaxnreg draws on the launch's registers");
 constexpr int MAX_STAGES = 8, MAX_ACC = 4;
-constexpr int AHEAD = 8;                    // blocks of K whose scales are on their way
+constexpr int AHEAD = 3;                    // blocks of K whose scales are on their way
 constexpr int STORE_BYTES = 4096;           // of a warp: 32 rows of 128 bytes
 constexpr int ROW_GROUP = 8;                // row tiles that are taken together
 
@@ -37,7 +38,7 @@ struct Params {
     const float *x_scales, *w_scales, *bias;
     void *y;
     long long x_scale_stride, w_scale_stride, y_stride;
-    int rows, outputs, kblocks, row_tiles, col_tiles, y_type, act, stages;
+    int rows, outputs, kblocks, row_tiles, col_tiles, y_type, act;
     int mapped;             // the result goes out by tensor-map stores
 };
 
@@ -55,11 +56,11 @@ __device__ __forceinline__ void commit_pair(uint32_t bar)
 {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((unsigned short)3) : "memory");
 }
-__device__ __forceinline__ void arrive_at(uint32_t remote) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory"); }
-__device__ __forceinline__ void scale_copy(uint32_t dst, const float *src, bool there)
-{
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
-}
+// Relaxed: what it says is that tensor memory has been read, which the tcgen05 fence before it orders.  A release would wait for the scale copies
+// that the thread has under way (1000 cycles a block of K).
+__device__ __forceinline__ void arrive_at(uint32_t remote) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory"); }
+constexpr int FIXED_BYTES = 2048 + SUM_WARPS * STORE_BYTES;             // alignment slack, barriers, store boxes
+constexpr int stages_for(int bn) { return std::min(MAX_STAGES, (SMEM_LIMIT - FIXED_BYTES) / ((BM + bn / 2) * BK)); }
 
 struct Tile { int row, col; };
 __device__ __forceinline__ Tile tile_at(int t, const Params &q)
@@ -78,17 +79,17 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
                       const Params q, int *status)
 {
     extern __shared__ unsigned char smem_raw[];
-    constexpr int ACC = 512 / BN;
+    constexpr int ACC = 512 / BN;                            // accumulators in tensor memory
     constexpr int X_BYTES = BM * BK, W_BYTES = BN / 2 * BK, STAGE_BYTES = X_BYTES + W_BYTES;
     constexpr int COLS = BN / 2;                             // of a summing warp
     unsigned char *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     Shared *sh = reinterpret_cast<Shared *>(smem);
     const uint32_t store0 = smem_u32(smem) + 1024;                                  // a store box for each summing warp
-    const uint32_t scales0 = store0 + SUM_WARPS * STORE_BYTES;                      // [block of K][thread]: scale of the row, scale of the columns
-    const uint32_t ring0 = scales0 + AHEAD * SUM_WARPS * 32 * 8;
+    const uint32_t ring0 = store0 + SUM_WARPS * STORE_BYTES;
+    constexpr int S = stages_for(BN);
     static_assert(sizeof(Shared) <= 1024, "barrier block");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int S = q.stages, kblocks = q.kblocks;
+    const int kblocks = q.kblocks;
     const uint32_t rank = cluster_rank();
     const int tiles = q.row_tiles * q.col_tiles, first = blockIdx.x >> 1, step = gridDim.x >> 1;
     int *abort_flag = &sh->abort_flag;
@@ -114,23 +115,26 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
     if(warp < WARP_SUM0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ISSUE));
         if(warp == WARP_COPY && lane == 0) {
-            uint32_t it = 0;
+            uint32_t s = 0, phase = 1, count = 0;
             bool live = true;
+            const uint32_t full0 = place_in(smem_u32(&sh->full[0]), 0), empty0 = smem_u32(&sh->empty[0]);
             for(int t = first; t < tiles && live; t += step) {
                 const Tile w = tile_at(t, q);
                 const int x_row = w.row * 2 * BM + int(rank) * BM, w_row = w.col * BN + int(rank) * (BN / 2);
-                for(int kb = 0; kb < kblocks; kb++, it++) {
-                    const int s = it % S;
-                    if(!mbar_wait(&sh->empty[s], ((it / S) & 1) ^ 1, abort_flag, status, SIP_EMPTY)) { live = false; break; }
-                    const uint32_t bar = place_in(smem_u32(&sh->full[s]), 0);
+                #pragma unroll 1
+                for(int kb = 0; kb < kblocks; kb++) {
+                    if(!mbar_wait(empty0 + 8 * s, phase, abort_flag, status, SIP_EMPTY)) { live = false; break; }
+                    const uint32_t slot = ring0 + s * STAGE_BYTES, bar = full0 + 8 * s;
                     if(rank == 0) mbar_arrive_expect_tx(&sh->full[s], 2 * STAGE_BYTES);
-                    tma_load_pair(ring0 + s * STAGE_BYTES, &tm_x, kb * BK, x_row, bar);
-                    tma_load_pair(ring0 + s * STAGE_BYTES + X_BYTES, &tm_w, kb * BK, w_row, bar);
+                    tma_load_pair(slot, &tm_x, kb * BK, x_row, bar);
+                    tma_load_pair(slot + X_BYTES, &tm_w, kb * BK, w_row, bar);
+                    count++;
+                    if(++s == S) { s = 0; phase ^= 1; }
                 }
             }
             // nothing may still be on its way into shared memory when the blocks end (the other block waits for this one below)
             if(rank == 0)
-                for(uint32_t n = it > uint32_t(S) ? it - S : 0; n < it; n++) {
+                for(uint32_t n = count > uint32_t(S) ? count - S : 0; n < count; n++) {
                     const long long t0 = global_ns();
                     while(!mbar_try_wait(&sh->full[n % S], (n / S) & 1)) {
                         __nanosleep(256);
@@ -141,73 +145,65 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
         else if(warp == WARP_MMA && lane == 0 && rank == 0) {
             constexpr uint32_t IDESC = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(2 * BM >> 4) << 24);     // fp32 sums of e4m3, K-major, M 256
             constexpr uint64_t DESC_HI = uint64_t((1024u >> 4) | (1u << 14) | (2u << 29)) << 32;   // 8-row groups 1024 bytes apart, version 1, SWIZZLE_128B
-            uint32_t it = 0;
-            bool live = true;
-            for(int t = first; t < tiles && live; t += step)
-                for(int kb = 0; kb < kblocks; kb++, it++) {
-                    const int s = it % S, b = it % ACC;
-                    if(!mbar_wait(&sh->acc_empty[b], ((it / ACC) & 1) ^ 1, abort_flag, status, SIP_ACC_EMPTY)) { live = false; break; }
-                    if(!mbar_wait(&sh->full[s], (it / S) & 1, abort_flag, status, SIP_FULL)) { live = false; break; }
-                    tc_fence_after();
-                    const uint32_t base = (((ring0 + s * STAGE_BYTES) & 0x3FFFF) >> 4) | (1u << 16);
-                    const uint64_t xd = DESC_HI | base, wd = DESC_HI | (base + (X_BYTES >> 4));
-                    #pragma unroll
-                    for(int j = 0; j < 4; j++)
-                        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                                     "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-                                     ::"r"(tmem_base + b * BN), "l"(xd + 2 * j), "l"(wd + 2 * j), "r"(IDESC), "r"(j) : "memory");
-                    commit_pair(smem_u32(&sh->empty[s]));
-                    commit_pair(smem_u32(&sh->acc_full[b]));
-                }
+            const uint32_t ring = ((ring0 & 0x3FFFF) >> 4) | (1u << 16);
+            const uint32_t full0 = smem_u32(&sh->full[0]), empty0 = smem_u32(&sh->empty[0]), acc_full0 = smem_u32(&sh->acc_full[0]), acc_empty0 = smem_u32(&sh->acc_empty[0]);
+            uint32_t s = 0, phase = 0, b = 0, b_phase = 1;
+            const long long total = (long long)((tiles - first + step - 1) / step) * kblocks;
+            #pragma unroll 1
+            for(long long it = 0; it < total; it++) {
+                // (the operands have been there for a while; the accumulator is what is waited for)
+                if(!mbar_wait(full0 + 8 * s, phase, abort_flag, status, SIP_FULL)) break;
+                const uint32_t xd = ring + s * (STAGE_BYTES >> 4), wd = xd + (X_BYTES >> 4), d = tmem_base + b * BN;
+                if(!mbar_wait(acc_empty0 + 8 * b, b_phase, abort_flag, status, SIP_ACC_EMPTY)) break;
+                tc_fence_after();
+                #pragma unroll
+                for(int j = 0; j < 4; j++)
+                    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                                 "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                                 ::"r"(d), "l"(DESC_HI | (xd + 2 * j)), "l"(DESC_HI | (wd + 2 * j)), "r"(IDESC), "r"(j) : "memory");
+                commit_pair(acc_full0 + 8 * b);
+                commit_pair(empty0 + 8 * s);
+                if(++s == S) { s = 0; phase ^= 1; }
+                if(++b == ACC) { b = 0; b_phase ^= 1; }
+            }
         }
     }
     else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SUM));
         const int me = warp - WARP_SUM0, quad = warp & 3, half = me >> 2;
-        const uint32_t my_scales = scales0 + (me * 32 + lane) * 8, my_store = store0 + me * STORE_BYTES;
-        const uint32_t empty0 = place_in(smem_u32(&sh->acc_empty[0]), 0);
+        const uint32_t my_store = store0 + me * STORE_BYTES;
+        const uint32_t acc_empty0 = place_in(smem_u32(&sh->acc_empty[0]), 0), acc_full0 = smem_u32(&sh->acc_full[0]);
         const float2 clamp = act_clamp(q.act);
         const int oblocks = (q.outputs + SCALE_BLOCK - 1) / SCALE_BLOCK;
-        uint32_t it = 0;
+        uint32_t b = 0, b_phase = 0;
         bool live = true;
-        // the scales of block kb of a tile: one group of asynchronous copies, empty beyond the last block
-        const float *xs = q.x_scales, *ws = q.w_scales;
-        bool xs_in = false, ws_in = false;
+        // Scales of the row and of the columns, AHEAD blocks of K before their use; zero beyond the matrices.
+        const float *xs = nullptr, *ws = nullptr;
+        float x_next[AHEAD], w_next[AHEAD];
+        auto ask = [&](int i, int kb) {
+            x_next[i] = xs && kb < kblocks ? ld_plain(xs + kb * q.x_scale_stride) : 0.0f;
+            w_next[i] = ws && kb < kblocks ? ld_plain(ws + kb) : 0.0f;
+        };
         auto aim = [&](int t) {
             const Tile w = tile_at(t, q);
             const int row = w.row * 2 * BM + int(rank) * BM + quad * 32 + lane, block = (w.col * BN + half * COLS) / SCALE_BLOCK;
-            xs_in = row < q.rows;
-            ws_in = block < oblocks;
-            xs = q.x_scales + (xs_in ? row : 0);
-            ws = q.w_scales + (ws_in ? block * q.w_scale_stride : 0);
+            xs = row < q.rows ? q.x_scales + row : nullptr;
+            ws = block < oblocks ? q.w_scales + block * q.w_scale_stride : nullptr;
+            #pragma unroll
+            for(int i = 0; i < AHEAD; i++) ask(i, i);
         };
-        auto ask = [&](int kb) {
-            if(kb < kblocks) {
-                const uint32_t dst = my_scales + (kb % AHEAD) * (SUM_WARPS * 32 * 8);
-                scale_copy(dst, xs + kb * q.x_scale_stride, xs_in);
-                scale_copy(dst + 4, ws + kb, ws_in);
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
-        if(first < tiles) {
-            aim(first);
-            for(int kb = 0; kb < AHEAD; kb++) ask(kb);
-        }
+        if(first < tiles) aim(first);
         for(int t = first; t < tiles && live; t += step) {
             float acc[COLS];
             #pragma unroll
             for(int j = 0; j < COLS; j++) acc[j] = 0.0f;
             #pragma unroll 1
-            for(int kb = 0; kb < kblocks; kb++, it++) {
-                const int b = it % ACC;
-                asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
-                float2 s2;
-                asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(s2.x), "=f"(s2.y) : "r"(my_scales + (kb % AHEAD) * (SUM_WARPS * 32 * 8)) : "memory");
-                // (written out: it keeps the copy into the same place, asked for below, behind the loads)
-                float s;
-                asm volatile("mul.f32 %0, %1, %2;" : "=f"(s) : "f"(s2.x), "f"(s2.y) : "memory");
-                if(!warp_wait(&sh->acc_full[b], (it / ACC) & 1, abort_flag, status, SIP_ACC_FULL, lane)) { live = false; break; }
-                ask(kb + AHEAD);
+            for(int kb = 0; kb < kblocks; kb++) {
+                const float s = x_next[0] * w_next[0];
+                #pragma unroll
+                for(int i = 0; i + 1 < AHEAD; i++) { x_next[i] = x_next[i + 1]; w_next[i] = w_next[i + 1]; }
+                ask(AHEAD - 1, kb + AHEAD);
+                if(!warp_wait(acc_full0 + 8 * b, b_phase, abort_flag, status, SIP_ACC_FULL, lane)) { live = false; break; }
                 tc_fence_after();
                 const uint32_t taddr = tmem_base + (uint32_t(quad * 32) << 16) + b * BN + half * COLS;
                 uint32_t v[2][32];
@@ -219,18 +215,16 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
                     else {
                         tc_fence_before();
                         __syncwarp();
-                        if(lane == 0) arrive_at(empty0 + 8 * b);
+                        if(lane == 0) arrive_at(acc_empty0 + 8 * b);
                     }
                     #pragma unroll
                     for(int j = 0; j < 32; j++) acc[g * 32 + j] = fmaf(__uint_as_float(v[g & 1][j]), s, acc[g * 32 + j]);
                 }
+                if(++b == ACC) { b = 0; b_phase ^= 1; }
             }
             if(!live) break;
             const Tile w = tile_at(t, q);
-            if(t + step < tiles) {                           // the next tile's first scales, under this one's way out
-                aim(t + step);
-                for(int kb = 0; kb < AHEAD; kb++) ask(kb);
-            }
+            if(t + step < tiles) aim(t + step);              // the next tile's first scales, under this one's way out
             // ---- bias, activation, out
             const int row0 = w.row * 2 * BM + int(rank) * BM + quad * 32, col0 = w.col * BN + half * COLS;
             if(row0 >= q.rows || col0 >= q.outputs) continue;
@@ -332,7 +326,6 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
                 }
             }
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
         if(lane == 0) bulk_wait_group<0>();
     }
 
@@ -380,10 +373,8 @@ template<int BN> dlp_status launch_bn(const Problem &p, cudaStream_t stream)
     if(st == DLP_OK) st = encode_operand(mw, p.w, p.w_stride, p.outputs, p.inputs, BN / 2);
     if(st == DLP_OK && q.mapped) st = encode_result(my, p);
     if(st != DLP_OK) return st;
-    const int fixed = 2048 + SUM_WARPS * STORE_BYTES + AHEAD * SUM_WARPS * 32 * 8, stage = (BM + BN / 2) * BK;
-    q.stages = std::min(MAX_STAGES, (SMEM_LIMIT - fixed) / stage);
     const int tiles = q.row_tiles * q.col_tiles, pairs = std::min(tiles, sm_count() / 2);
-    DLP_LAUNCH_PDL(launch_pdl_cluster(few_items(2 * tiles), 2, scaled_ip_pair_kernel<BN>, 2 * pairs, NUM_THREADS, fixed + q.stages * stage, stream, mx, mw, my, q,
+    DLP_LAUNCH_PDL(launch_pdl_cluster(few_items(2 * tiles), 2, scaled_ip_pair_kernel<BN>, 2 * pairs, NUM_THREADS, FIXED_BYTES + stages_for(BN) * (BM + BN / 2) * BK, stream, mx, mw, my, q,
                                       status), "scaled_ip_pair_kernel");
     return DLP_OK;
 }
