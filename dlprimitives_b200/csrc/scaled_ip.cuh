@@ -12,7 +12,7 @@ using namespace tc;
 
 constexpr int BM = 128, BK = 128;           // rows of an operand tile; a block of K, one 128-byte row of the swizzled operand tiles
 constexpr int SMEM_LIMIT = 227 * 1024;
-enum { SIP_EMPTY = 501, SIP_FULL = 502, SIP_ACC_EMPTY = 503, SIP_ACC_FULL = 504, SIP_DRAIN = 505 };
+enum { SIP_EMPTY = 501, SIP_FULL = 502, SIP_ACC_EMPTY = 503, SIP_ACC_FULL = 504, SIP_DRAIN = 505, SIP_SCALE_EMPTY = 506, SIP_SCALE_FULL = 507 };
 
 struct Problem {
     const void *x, *w;

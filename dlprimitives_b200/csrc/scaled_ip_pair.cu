@@ -7,8 +7,8 @@
 // pair reads a row of w once where two single SMs would read it twice.
 //   * one warp per SM issues the tensor-map copies of its half; both halves' bytes are counted on the leader's barrier;
 //   * one thread of the leader issues the MMAs of the pair; its commits go to both SMs;
-//   * eight warps per SM sum: a quarter of the rows and half of the columns each.  Each thread loads its scales
-//     three blocks ahead.  They store through shared memory and tensor-map stores.
+//   * eight warps per SM sum: a quarter of the rows and half of the columns each, and store through shared memory and tensor-map stores;
+//   * two warps per SM bring in the scales, eight blocks of K at a time, and leave their products in shared memory.
 // Tiles are taken in turn (persistent blocks), eight row tiles at a time down the columns, so that what the SMs read at one time stays in L2.
 // Every wait is bounded.
 #define DLP_INLINE_WAITS
@@ -19,17 +19,18 @@ namespace dlp {
 namespace sip {
 namespace {
 
-constexpr int WARP_COPY = 0, WARP_MMA = 1, WARP_SUM0 = 4;
+constexpr int WARP_COPY = 0, WARP_MMA = 1, WARP_SCALE0 = 2, WARP_SUM0 = 4;
 constexpr int NUM_THREADS = 384, SUM_WARPS = 8;
-constexpr int REGS_LAUNCH = 168, REGS_ISSUE = 40, REGS_SUM = 232;
+constexpr int REGS_LAUNCH = 168, REGS_ISSUE = 56, REGS_SUM = 224;
 static_assert(REGS_ISSUE + 2 * REGS_SUM <= 3 * REGS_LAUNCH, "setmaxnreg draws on the launch's registers");
 constexpr int MAX_STAGES = 8, MAX_ACC = 4;
-constexpr int AHEAD = 3;                    // blocks of K whose scales are on their way
-constexpr int STORE_BYTES = 4096;           // of a warp: 32 rows of 128 bytes
+constexpr int CHUNK = 8;                    // blocks of K whose scales are brought in together
+constexpr int SCALE_BYTES = CHUNK * 2 * BM * 4;             // [block][half of the columns][row]
+constexpr int STORE_BYTES = 2 * 4096;       // of a warp: two boxes of 32 rows of 128 bytes
 constexpr int ROW_GROUP = 8;                // row tiles that are taken together
 
 struct Shared {
-    unsigned long long full[MAX_STAGES], empty[MAX_STAGES], acc_full[MAX_ACC], acc_empty[MAX_ACC], drain;
+    unsigned long long full[MAX_STAGES], empty[MAX_STAGES], acc_full[MAX_ACC], acc_empty[MAX_ACC], scale_full[2], scale_empty[2], drain;
     uint32_t tmem_base;
     int abort_flag;
 };
@@ -59,7 +60,7 @@ __device__ __forceinline__ void commit_pair(uint32_t bar)
 // Relaxed: what it says is that tensor memory has been read, which the tcgen05 fence before it orders.  A release would wait for the scale copies
 // that the thread has under way (1000 cycles a block of K).
 __device__ __forceinline__ void arrive_at(uint32_t remote) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory"); }
-constexpr int FIXED_BYTES = 2048 + SUM_WARPS * STORE_BYTES;             // alignment slack, barriers, store boxes
+constexpr int FIXED_BYTES = 2048 + SUM_WARPS * STORE_BYTES + 2 * SCALE_BYTES;       // alignment slack, barriers, store boxes, scales
 constexpr int stages_for(int bn) { return std::min(MAX_STAGES, (SMEM_LIMIT - FIXED_BYTES) / ((BM + bn / 2) * BK)); }
 
 struct Tile { int row, col; };
@@ -85,7 +86,7 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
     unsigned char *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     Shared *sh = reinterpret_cast<Shared *>(smem);
     const uint32_t store0 = smem_u32(smem) + 1024;                                  // a store box for each summing warp
-    const uint32_t ring0 = store0 + SUM_WARPS * STORE_BYTES;
+    const uint32_t scales0 = store0 + SUM_WARPS * STORE_BYTES, ring0 = scales0 + 2 * SCALE_BYTES;
     constexpr int S = stages_for(BN);
     static_assert(sizeof(Shared) <= 1024, "barrier block");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -97,6 +98,7 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
     if(threadIdx.x == 0) {
         for(int s = 0; s < MAX_STAGES; s++) { mbar_init(&sh->full[s], 1); mbar_init(&sh->empty[s], 1); }
         for(int a = 0; a < MAX_ACC; a++) { mbar_init(&sh->acc_full[a], 1); mbar_init(&sh->acc_empty[a], 2 * SUM_WARPS); }
+        for(int a = 0; a < 2; a++) { mbar_init(&sh->scale_full[a], 2); mbar_init(&sh->scale_empty[a], SUM_WARPS); }
         mbar_init(&sh->drain, 1);
         sh->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -167,6 +169,47 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
                 if(++b == ACC) { b = 0; b_phase ^= 1; }
             }
         }
+        else if(warp >= WARP_SCALE0) {
+            // products of the two scales, a chunk of blocks of K at a time; a lane has two of the tile's rows
+            const int r0 = (warp - WARP_SCALE0) * 64 + lane, oblocks = (q.outputs + SCALE_BLOCK - 1) / SCALE_BLOCK;
+            uint32_t slot = 0, phase = 1;
+            bool live = true;
+            for(int t = first; t < tiles && live; t += step) {
+                const Tile w = tile_at(t, q);
+                const int row = w.row * 2 * BM + int(rank) * BM + r0, block0 = w.col * BN / SCALE_BLOCK, block1 = (w.col * BN + COLS) / SCALE_BLOCK;
+                const bool in0 = row < q.rows, in1 = row + 32 < q.rows, cols0 = block0 < oblocks, cols1 = block1 < oblocks;
+                const float *xs = q.x_scales + row, *ws0 = q.w_scales + block0 * q.w_scale_stride, *ws1 = q.w_scales + block1 * q.w_scale_stride;
+                #pragma unroll 1
+                for(int kb0 = 0; kb0 < kblocks; kb0 += CHUNK) {
+                    if(!warp_wait(&sh->scale_empty[slot], phase, abort_flag, status, SIP_SCALE_EMPTY, lane)) { live = false; break; }
+                    #pragma unroll
+                    for(int i0 = 0; i0 < CHUNK; i0 += 4) {
+                        float x0[4], x1[4], w0[4], w1[4];
+                        #pragma unroll
+                        for(int i = 0; i < 4; i++) {
+                            const int kb = kb0 + i0 + i;
+                            const bool there = kb < kblocks;
+                            x0[i] = there && in0 ? ld_plain(xs + kb * q.x_scale_stride) : 0.0f;
+                            x1[i] = there && in1 ? ld_plain(xs + kb * q.x_scale_stride + 32) : 0.0f;
+                            w0[i] = there && cols0 ? ld_plain(ws0 + kb) : 0.0f;
+                            w1[i] = there && cols1 ? ld_plain(ws1 + kb) : 0.0f;
+                        }
+                        #pragma unroll
+                        for(int i = 0; i < 4; i++) {
+                            const uint32_t at = scales0 + slot * SCALE_BYTES + ((i0 + i) * 2 * BM + r0) * 4;
+                            asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(x0[i] * w0[i]) : "memory");
+                            asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + 128), "f"(x1[i] * w0[i]) : "memory");
+                            asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + BM * 4), "f"(x0[i] * w1[i]) : "memory");
+                            asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + BM * 4 + 128), "f"(x1[i] * w1[i]) : "memory");
+                        }
+                    }
+                    __syncwarp();
+                    if(lane == 0) mbar_arrive(&sh->scale_full[slot]);
+                    slot ^= 1;
+                    if(slot == 0) phase ^= 1;
+                }
+            }
+        }
     }
     else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SUM));
@@ -174,36 +217,26 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
         const uint32_t my_store = store0 + me * STORE_BYTES;
         const uint32_t acc_empty0 = place_in(smem_u32(&sh->acc_empty[0]), 0), acc_full0 = smem_u32(&sh->acc_full[0]);
         const float2 clamp = act_clamp(q.act);
-        const int oblocks = (q.outputs + SCALE_BLOCK - 1) / SCALE_BLOCK;
-        uint32_t b = 0, b_phase = 0;
+        const uint32_t my_scales = scales0 + (half * BM + quad * 32 + lane) * 4, scale_empty0 = smem_u32(&sh->scale_empty[0]);
+        uint32_t b = 0, b_phase = 0, slot = 1, s_phase = 1, store_at = my_store;
         bool live = true;
-        // Scales of the row and of the columns, AHEAD blocks of K before their use; zero beyond the matrices.
-        const float *xs = nullptr, *ws = nullptr;
-        float x_next[AHEAD], w_next[AHEAD];
-        auto ask = [&](int i, int kb) {
-            x_next[i] = xs && kb < kblocks ? ld_plain(xs + kb * q.x_scale_stride) : 0.0f;
-            w_next[i] = ws && kb < kblocks ? ld_plain(ws + kb) : 0.0f;
-        };
-        auto aim = [&](int t) {
-            const Tile w = tile_at(t, q);
-            const int row = w.row * 2 * BM + int(rank) * BM + quad * 32 + lane, block = (w.col * BN + half * COLS) / SCALE_BLOCK;
-            xs = row < q.rows ? q.x_scales + row : nullptr;
-            ws = block < oblocks ? q.w_scales + block * q.w_scale_stride : nullptr;
-            #pragma unroll
-            for(int i = 0; i < AHEAD; i++) ask(i, i);
-        };
-        if(first < tiles) aim(first);
         for(int t = first; t < tiles && live; t += step) {
             float acc[COLS];
             #pragma unroll
             for(int j = 0; j < COLS; j++) acc[j] = 0.0f;
             #pragma unroll 1
             for(int kb = 0; kb < kblocks; kb++) {
-                const float s = x_next[0] * w_next[0];
-                #pragma unroll
-                for(int i = 0; i + 1 < AHEAD; i++) { x_next[i] = x_next[i + 1]; w_next[i] = w_next[i + 1]; }
-                ask(AHEAD - 1, kb + AHEAD);
-                if(!warp_wait(acc_full0 + 8 * b, b_phase, abort_flag, status, SIP_ACC_FULL, lane)) { live = false; break; }
+                const int in = kb % CHUNK;
+                if(in == 0) {
+                    slot ^= 1;
+                    if(slot == 0) s_phase ^= 1;
+                    if(!warp_wait(&sh->scale_full[slot], s_phase, abort_flag, status, SIP_SCALE_FULL, lane)) { live = false; break; }
+                }
+                float s;
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(s) : "r"(my_scales + slot * SCALE_BYTES + in * (2 * BM * 4)) : "memory");
+                // (no vote: should the wait give up, what is read below means nothing, and the abort flag is seen at the next chunk)
+                if(lane == 0) mbar_wait(acc_full0 + 8 * b, b_phase, abort_flag, status, SIP_ACC_FULL);
+                __syncwarp();
                 tc_fence_after();
                 const uint32_t taddr = tmem_base + (uint32_t(quad * 32) << 16) + b * BN + half * COLS;
                 uint32_t v[2][32];
@@ -215,16 +248,19 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
                     else {
                         tc_fence_before();
                         __syncwarp();
-                        if(lane == 0) arrive_at(acc_empty0 + 8 * b);
+                        if(lane == 0) {
+                            arrive_at(acc_empty0 + 8 * b);
+                            if(in == CHUNK - 1 || kb + 1 == kblocks) mbar_arrive(scale_empty0 + 8 * slot);
+                        }
                     }
                     #pragma unroll
                     for(int j = 0; j < 32; j++) acc[g * 32 + j] = fmaf(__uint_as_float(v[g & 1][j]), s, acc[g * 32 + j]);
                 }
                 if(++b == ACC) { b = 0; b_phase ^= 1; }
             }
+            live = live && !*(volatile int *)abort_flag;
             if(!live) break;
             const Tile w = tile_at(t, q);
-            if(t + step < tiles) aim(t + step);              // the next tile's first scales, under this one's way out
             // ---- bias, activation, out
             const int row0 = w.row * 2 * BM + int(rank) * BM + quad * 32, col0 = w.col * BN + half * COLS;
             if(row0 >= q.rows || col0 >= q.outputs) continue;
@@ -237,7 +273,8 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
                     for(int j = 0; j < 32; j++) acc[g * 32 + j] += __shfl_sync(0xffffffffu, bias_g, j);
                 }
             }
-            if(act_is_clamp(q.act)) {
+            if(q.act == DLP_ACT_IDENTITY) {}
+            else if(act_is_clamp(q.act)) {
                 #pragma unroll
                 for(int j = 0; j < COLS; j++) acc[j] = fminf(fmaxf(acc[j], clamp.x), clamp.y);
             }
@@ -270,18 +307,19 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
             // describes, are stored by the warp, a row at a time.
             auto box = [&](const uint32_t (&v)[32], int col, int size) {
                 if(col >= q.outputs) return;
-                if(lane == 0) bulk_wait_group_read<0>();
+                store_at = store_at == my_store ? my_store + 4096 : my_store;
+                if(lane == 0) bulk_wait_group_read<1>();         // this box's last store is two back
                 __syncwarp();
                 #pragma unroll
                 for(int c = 0; c < 8; c++)
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(my_store + lane * 128 + ((c ^ (lane & 7)) << 4)), "r"(v[4 * c]), "r"(v[4 * c + 1]),
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(store_at + lane * 128 + ((c ^ (lane & 7)) << 4)), "r"(v[4 * c]), "r"(v[4 * c + 1]),
                                  "r"(v[4 * c + 2]), "r"(v[4 * c + 3]) : "memory");
                 const int bytes = min(q.outputs - col, 128 / size) * size;
                 if(q.mapped && bytes % 16 == 0) {
                     fence_proxy_async_shared();
                     __syncwarp();
                     if(lane == 0) {
-                        tma_store_2d(&tm_y, col, row0, my_store);
+                        tma_store_2d(&tm_y, col, row0, store_at);
                         bulk_commit_group();
                     }
                     return;
@@ -292,7 +330,7 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
                 #pragma unroll 1
                 for(int r = 0; r < rows; r++, at += q.y_stride * size) {
                     uint32_t word;
-                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(word) : "r"(my_store + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) : "memory");
+                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(word) : "r"(store_at + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) : "memory");
                     if(size == 4) {
                         if(lane * 4 < bytes) *reinterpret_cast<uint32_t *>(at) = word;
                     }
@@ -302,6 +340,7 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
                     }
                 }
                 __syncwarp();
+                if(lane == 0) bulk_commit_group();           // an empty one: the waits count boxes
             };
             if(q.y_type == DLP_TYPE_F32) {
                 #pragma unroll
