@@ -6,6 +6,7 @@ if the library is missing this module raises at import, and every call needs CUD
 """
 import ctypes as C
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libdlprim_b200_cuda.so")
@@ -44,6 +45,27 @@ class GemmDesc(C.Structure):
 class IpDesc(C.Structure):
     _fields_ = [("inputs", C.c_int), ("outputs", C.c_int), ("optimal_batch_size", C.c_int), ("bias", C.c_int),
                 ("activation", C.c_int), ("math_mode", C.c_int)]
+
+
+def _fields(addresses, longs, ints, floats=""):
+    return ([(n, C.c_void_p) for n in addresses.split()] + [(n, C.c_longlong) for n in longs.split()] + [(n, C.c_int) for n in ints.split()] +
+            [(n, C.c_float) for n in floats.split()])
+
+
+class RmsNormArgs(C.Structure):
+    _fields_ = _fields("x residual weight total y scales", "x_stride residual_stride total_stride y_stride scale_stride", "rows cols type y_type", "eps")
+
+
+class QuantizeArgs(C.Structure):
+    _fields_ = _fields("x q scales", "x_stride q_stride scale_stride", "rows cols type gate block_rows")
+
+
+class ScaledIpArgs(C.Structure):
+    _fields_ = _fields("x x_scales w w_scales bias y", "x_stride x_scale_stride w_stride w_scale_stride y_stride", "rows inputs outputs y_type activation")
+
+
+class SampleArgs(C.Structure):
+    _fields_ = _fields("logits temperature top_k top_p min_p u tokens", "stride", "rows classes type")
 
 
 # every symbol include/dlp_cuda.h declares: name -> (restype, argtypes)
@@ -94,10 +116,10 @@ SYMBOLS = {
     "dlp_activation_fwd": (_i, [_fp, _fp, _sz, _i, _vp]),
     "dlp_softmax_fwd": (_i, [_fp, _fp, _i, _i, _i, _i, _vp]),
     "dlp_batchnorm_inference_fwd": (_i, [_fp, _fp, _i, _i, _i, _f, _fp, _fp, _fp, _fp, _vp]),
-    "dlp_rms_norm_fwd": (_i, [_vp, _ll, _vp, _ll, _vp, _ll, _vp, _i, _vp, _ll, _i, _vp, _ll, _i, _i, _f, _vp]),
-    "dlp_quantize_fwd": (_i, [_vp, _ll, _i, _i, _vp, _ll, _vp, _ll, _i, _i, _i, _vp]),
-    "dlp_scaled_ip_fwd": (_i, [_vp, _ll, _vp, _ll, _vp, _ll, _vp, _ll, _vp, _vp, _ll, _i, _i, _i, _i, _i, _vp]),
-    "dlp_sample_fwd": (_i, [_vp, _ll, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "dlp_rms_norm_fwd": (_i, [_vp, _vp]),
+    "dlp_quantize_fwd": (_i, [_vp, _vp]),
+    "dlp_scaled_ip_fwd": (_i, [_vp, _vp]),
+    "dlp_sample_fwd": (_i, [_vp, _vp]),
 }
 
 _lib = None
@@ -390,91 +412,124 @@ def batchnorm_inference(x, y, mean, var, gamma=None, beta=None, eps=1e-5, stream
 
 
 # ---- operators with typed operands: from a hidden state to a token ---------------------------------
+# These run once for every layer and token, on tensors that take a few microseconds, so the calls here are kept short: arguments go over as a
+# packed structure (a tenth of the time of as many separate ones), and a tensor that is as expected costs one look at each of its properties.
 GATES = {"none": 0, "silu": 1, "gelu": 2}
-TYPES = {"float32": 0, "float16": 1, "bfloat16": 2, "float8_e4m3fn": 3}
 SCALE_BLOCK = 128
 SAMPLE_MAX_CLASSES = 1 << 22
-_type_codes = {}
 
 
-def _type(t):
+def _packer(cls):
+    """Packs the fields' values, in their order, into the structure's bytes."""
+    size = {C.c_void_p: "P", C.c_longlong: "q", C.c_int: "i", C.c_float: "f"}
+    form = struct.Struct("@" + "".join(size[t] for _, t in cls._fields_) + "0q")
+    assert form.size == C.sizeof(cls)
+    return form.pack
+
+
+_pack_rms_norm, _pack_quantize, _pack_scaled_ip, _pack_sample = map(_packer, (RmsNormArgs, QuantizeArgs, ScaledIpArgs, SampleArgs))
+
+
+class _Torch:
+    """What the calls below need of torch, looked up when the first of them is made."""
+    codes = {}
+
+    @classmethod
+    def load(cls):
+        import torch
+        cls.f32, cls.e4m3, cls.i32 = torch.float32, torch.float8_e4m3fn, torch.int32
+        cls.current_device, cls.raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+        cls.codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.float8_e4m3fn: 3}
+
+
+def _code(t, name):
     """DLP_TYPE_* of a tensor."""
-    code = _type_codes.get(t.dtype)
+    code = _Torch.codes.get(t.dtype)
     if code is None:
-        code = TYPES.get(str(t.dtype).replace("torch.", ""))
+        _Torch.load()
+        code = _Torch.codes.get(t.dtype)
         if code is None:
-            raise ValueError("fp32, fp16, bf16 or e4m3 tensors expected, not %s" % t.dtype)
-        _type_codes[t.dtype] = code
+            raise ValueError("%s: fp32, fp16, bf16 or e4m3 expected, not %s" % (name, t.dtype))
     return code
 
 
-def _typed(t, code, shape, name, device):
-    """(address, row stride) of a vector or matrix of this shape, with unit stride along its rows, on the current device."""
-    if tuple(t.shape) != shape:
-        raise ValueError("%s: expected shape %s, not %s" % (name, list(shape), list(t.shape)))
-    if code >= 0 and _type(t) != code:
-        raise ValueError("%s: another type was expected than %s" % (name, t.dtype))
-    if t.get_device() != device:
-        raise ValueError("%s is not on the current device" % name)
-    stride = t.stride()
-    if stride[-1] != 1 and shape[-1] > 1:
+def _device_of(t):
+    dev = t.get_device()
+    if dev < 0 or dev != _Torch.current_device():
+        raise ValueError("the tensors must be on the current CUDA device")
+    return dev
+
+
+def _tensor(t, dtype, shape, device, name):
+    """(address, row stride) of a vector or matrix that has to be of this type and shape, on this device, and contiguous along its last dimension."""
+    if t.dtype is dtype and t.shape == shape and t.get_device() == device:
+        if t.is_contiguous():
+            return t.data_ptr(), shape[-1]
+        if len(shape) == 2:
+            rows, cols = t.stride()
+            if cols == 1 or shape[1] == 1:
+                return t.data_ptr(), rows
         raise ValueError("%s: rows must be contiguous" % name)
-    return t.data_ptr(), (stride[0] if len(shape) > 1 else 0)
+    raise ValueError("%s: expected %s %s on device %d, not %s %s on %s" % (name, dtype, list(shape), device, t.dtype, list(t.shape), t.device))
 
 
-def _device():
-    import torch
-    return torch.cuda.current_device()
+def _call(fn, args, stream, device):
+    status = fn(args, stream.cuda_stream if stream is not None else _Torch.raw_stream(device))
+    if status:
+        check(status)
 
 
 def rms_norm(x, weight, y, residual=None, total=None, scales=None, eps=1e-6, stream=None):
     """y = h / sqrt(mean(h^2) + eps) * weight with h = x + residual; total (optional) receives h.  An e4m3 y comes with scales
     [ceil(cols / 128), rows]."""
-    rows, cols = x.shape
-    dev, t, yt = _device(), _type(x), _type(y)
-    xp, xs = _typed(x, t, (rows, cols), "x", dev)
-    wp, _ = _typed(weight, t, (cols,), "weight", dev)
-    yp, ys = _typed(y, yt, (rows, cols), "y", dev)
-    rp, rs = _typed(residual, t, (rows, cols), "residual", dev) if residual is not None else (None, 0)
-    tp, ts = _typed(total, t, (rows, cols), "total", dev) if total is not None else (None, 0)
-    sp, ss = _typed(scales, 0, (-(-cols // SCALE_BLOCK), rows), "scales", dev) if scales is not None else (None, 0)
-    check(lib().dlp_rms_norm_fwd(xp, xs, rp, rs, tp, ts, wp, t, yp, ys, yt, sp, ss, rows, cols, eps, _stream(stream)))
+    shape = rows, cols = x.shape
+    code, y_code, dev, dtype = _code(x, "x"), _code(y, "y"), _device_of(x), x.dtype
+    xp, xs = _tensor(x, dtype, shape, dev, "x")
+    wp, _ = _tensor(weight, dtype, (cols,), dev, "weight")
+    yp, ys = _tensor(y, y.dtype, shape, dev, "y")
+    rp, rs = _tensor(residual, dtype, shape, dev, "residual") if residual is not None else (0, 0)
+    tp, ts = _tensor(total, dtype, shape, dev, "total") if total is not None else (0, 0)
+    sp, ss = _tensor(scales, _Torch.f32, ((cols + SCALE_BLOCK - 1) // SCALE_BLOCK, rows), dev, "scales") if scales is not None else (0, 0)
+    _call(lib().dlp_rms_norm_fwd, _pack_rms_norm(xp, rp, wp, tp, yp, sp, xs, rs, ts, ys, ss, rows, cols, code, y_code, eps), stream, dev)
 
 
 def quantize(x, q, scales, gate="none", block_rows=1, stream=None):
     """q [rows, cols] (e4m3) and scales: the 8-bit form of x, or of act(a) * b for x = [a | b] (gate "silu" or "gelu").  block_rows 1: scales
     [ceil(cols / 128), rows]; 128: [ceil(rows / 128), ceil(cols / 128)]."""
-    rows, cols = q.shape
-    dev, t, g = _device(), _type(x), GATES[gate]
-    xp, xs = _typed(x, t, (rows, 2 * cols if g else cols), "x", dev)
-    qp, qs = _typed(q, TYPES["float8_e4m3fn"], (rows, cols), "q", dev)
-    blocks = -(-cols // SCALE_BLOCK)
-    sp, ss = _typed(scales, 0, (blocks, rows) if block_rows == 1 else (-(-rows // SCALE_BLOCK), blocks), "scales", dev)
-    check(lib().dlp_quantize_fwd(xp, xs, t, g, qp, qs, sp, ss, block_rows, rows, cols, _stream(stream)))
+    shape = rows, cols = q.shape
+    code, g, dev = _code(x, "x"), GATES[gate], _device_of(x)
+    blocks = (cols + SCALE_BLOCK - 1) // SCALE_BLOCK
+    xp, xs = _tensor(x, x.dtype, (rows, 2 * cols) if g else shape, dev, "x")
+    qp, qs = _tensor(q, _Torch.e4m3, shape, dev, "q")
+    sp, ss = _tensor(scales, _Torch.f32, (blocks, rows) if block_rows == 1 else ((rows + SCALE_BLOCK - 1) // SCALE_BLOCK, blocks), dev, "scales")
+    _call(lib().dlp_quantize_fwd, _pack_quantize(xp, qp, sp, xs, qs, ss, rows, cols, code, g, block_rows), stream, dev)
 
 
 def scaled_inner_product(x, x_scales, w, w_scales, y, bias=None, activation="identity", stream=None):
     """y = act(x * w^T + bias) for 8-bit x [rows, inputs] in blocks of one row and w [outputs, inputs] in blocks of 128 x 128."""
     (rows, inputs), outputs = x.shape, w.shape[0]
-    dev, e4m3, yt, blocks = _device(), TYPES["float8_e4m3fn"], _type(y), -(-inputs // SCALE_BLOCK)
-    xp, xs = _typed(x, e4m3, (rows, inputs), "x", dev)
-    xsp, xss = _typed(x_scales, 0, (blocks, rows), "x_scales", dev)
-    wp, ws = _typed(w, e4m3, (outputs, inputs), "w", dev)
-    wsp, wss = _typed(w_scales, 0, (-(-outputs // SCALE_BLOCK), blocks), "w_scales", dev)
-    yp, ys = _typed(y, yt, (rows, outputs), "y", dev)
-    bp = _typed(bias, 0, (outputs,), "bias", dev)[0] if bias is not None else None
-    check(lib().dlp_scaled_ip_fwd(xp, xs, xsp, xss, wp, ws, wsp, wss, bp, yp, ys, yt, _act(activation), rows, inputs, outputs, _stream(stream)))
+    y_code, dev, blocks = _code(y, "y"), _device_of(x), (inputs + SCALE_BLOCK - 1) // SCALE_BLOCK
+    e4m3, f32 = _Torch.e4m3, _Torch.f32
+    xp, xs = _tensor(x, e4m3, (rows, inputs), dev, "x")
+    xsp, xss = _tensor(x_scales, f32, (blocks, rows), dev, "x_scales")
+    wp, ws = _tensor(w, e4m3, (outputs, inputs), dev, "w")
+    wsp, wss = _tensor(w_scales, f32, ((outputs + SCALE_BLOCK - 1) // SCALE_BLOCK, blocks), dev, "w_scales")
+    yp, ys = _tensor(y, y.dtype, (rows, outputs), dev, "y")
+    bp = _tensor(bias, f32, (outputs,), dev, "bias")[0] if bias is not None else 0
+    _call(lib().dlp_scaled_ip_fwd, _pack_scaled_ip(xp, xsp, wp, wsp, bp, yp, xs, xss, ws, wss, ys, rows, inputs, outputs, y_code, _act(activation)), stream,
+          dev)
 
 
 def sample(logits, u, tokens, temperature=None, top_k=None, top_p=None, min_p=None, stream=None):
     """tokens [rows] (int32): a class drawn from each row of logits with the row's random number u in [0, 1); -1 where every logit is
-    masked.  Settings are per-row vectors or None."""
-    import torch
+    masked.  Settings are per-row vectors (fp32; top_k int32) or None."""
     rows, classes = logits.shape
-    dev, t = _device(), _type(logits)
-    lp, ls = _typed(logits, t, (rows, classes), "logits", dev)
-    if tokens.dtype != torch.int32 or (top_k is not None and top_k.dtype != torch.int32):
-        raise ValueError("tokens and top_k are int32")
-    row = [None if v is None else _typed(v, code, (rows,), name, dev)[0] for v, code, name in (
-        (temperature, 0, "temperature"), (top_k, -1, "top_k"), (top_p, 0, "top_p"), (min_p, 0, "min_p"), (u, 0, "u"), (tokens, -1, "tokens"))]
-    check(lib().dlp_sample_fwd(lp, ls, t, rows, classes, *row, _stream(stream)))
+    code, dev, row = _code(logits, "logits"), _device_of(logits), (rows,)
+    f32, i32 = _Torch.f32, _Torch.i32
+    lp, ls = _tensor(logits, logits.dtype, (rows, classes), dev, "logits")
+    up, op = _tensor(u, f32, row, dev, "u")[0], _tensor(tokens, i32, row, dev, "tokens")[0]
+    tp = _tensor(temperature, f32, row, dev, "temperature")[0] if temperature is not None else 0
+    kp = _tensor(top_k, i32, row, dev, "top_k")[0] if top_k is not None else 0
+    pp = _tensor(top_p, f32, row, dev, "top_p")[0] if top_p is not None else 0
+    mp = _tensor(min_p, f32, row, dev, "min_p")[0] if min_p is not None else 0
+    _call(lib().dlp_sample_fwd, _pack_sample(lp, tp, kp, pp, mp, up, op, ls, rows, classes, code), stream, dev)

@@ -108,9 +108,10 @@ using namespace dlp;
 
 extern "C" {
 
-dlp_status dlp_quantize_fwd(const void *x, long long x_stride, int type, int gate, void *q, long long q_stride, float *scales,
-                            long long scale_stride, int block_rows, int rows, int cols, void *stream)
+dlp_status dlp_quantize_fwd(const dlp_quantize_args *args, void *stream)
 {
+    DLP_REQUIRE(args != nullptr, "null arguments");
+    const auto [x, q, scales, x_stride, q_stride, scale_stride, rows, cols, type, gate, block_rows] = *args;
     DLP_REQUIRE(rows >= 0 && cols > 0 && cols < (1 << 30), "bad shape");
     DLP_REQUIRE(is_real_type(type), "the input's type must be fp32, fp16 or bf16");
     DLP_REQUIRE(gate >= DLP_GATE_NONE && gate <= DLP_GATE_GELU, "unknown gate");

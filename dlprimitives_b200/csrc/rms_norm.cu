@@ -97,10 +97,10 @@ using namespace dlp;
 
 extern "C" {
 
-dlp_status dlp_rms_norm_fwd(const void *x, long long x_stride, const void *residual, long long residual_stride, void *total,
-                            long long total_stride, const void *weight, int type, void *y, long long y_stride, int y_type, float *scales,
-                            long long scale_stride, int rows, int cols, float eps, void *stream)
+dlp_status dlp_rms_norm_fwd(const dlp_rms_norm_args *args, void *stream)
 {
+    DLP_REQUIRE(args != nullptr, "null arguments");
+    const auto [x, residual, weight, total, y, scales, x_stride, residual_stride, total_stride, y_stride, scale_stride, rows, cols, type, y_type, eps] = *args;
     DLP_REQUIRE(rows >= 0 && cols > 0, "bad norm shape");
     DLP_REQUIRE(is_real_type(type), "the input's type must be fp32, fp16 or bf16");
     DLP_REQUIRE(is_real_type(y_type) || y_type == DLP_TYPE_E4M3, "unknown output type");
@@ -117,7 +117,7 @@ dlp_status dlp_rms_norm_fwd(const void *x, long long x_stride, const void *resid
                 (!total || aligned_to(total, size)) && (!scales || aligned_to(scales, 4)), "a tensor is not aligned to its elements");
     NormArgs a = { x, residual, weight, total, y, scales, x_stride, residual_stride, total_stride, y_stride, scale_stride, cols, y_type, eps };
     // 16-byte accesses (8 for the 8-bit output): every row and its end on such a boundary
-    const auto rows_on = [&](const void *p, long long stride, size_t element, size_t n) { return aligned_to(p, n) && (rows == 1 || stride * element % n == 0); };
+    const auto rows_on = [rows = args->rows](const void *p, long long stride, size_t element, size_t n) { return aligned_to(p, n) && (rows == 1 || stride * element % n == 0); };
     const bool vec = cols % 8 == 0 && rows_on(x, x_stride, size, 16) && aligned_to(weight, 16) && (!residual || rows_on(residual, residual_stride, size, 16)) &&
                      (!total || rows_on(total, total_stride, size, 16)) && rows_on(y, y_stride, y_size, y_type == DLP_TYPE_E4M3 ? 8 : 16);
     if(type == DLP_TYPE_F32) return launch_norm<float>(a, rows, vec, (cudaStream_t)stream);

@@ -581,9 +581,10 @@ using namespace dlp;
 
 extern "C" {
 
-dlp_status dlp_sample_fwd(const void *logits, long long stride, int type, int rows, int classes, const float *temperature, const int *top_k,
-                          const float *top_p, const float *min_p, const float *u, int *tokens, void *stream)
+dlp_status dlp_sample_fwd(const dlp_sample_args *args, void *stream)
 {
+    DLP_REQUIRE(args != nullptr, "null arguments");
+    const auto [logits, temperature, top_k, top_p, min_p, u, tokens, stride, rows, classes, type] = *args;
     DLP_REQUIRE(rows >= 0 && classes > 0 && classes <= DLP_SAMPLE_MAX_CLASSES, "bad shape");
     DLP_REQUIRE(is_real_type(type), "the logits' type must be fp32, fp16 or bf16");
     if(rows == 0) return DLP_OK;

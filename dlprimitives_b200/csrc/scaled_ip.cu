@@ -10,14 +10,13 @@
 //     added through distributed shared memory in a fixed order.
 // Every wait is bounded (device status word + abort flag).
 #include "scaled_ip.cuh"
-#include <cstring>
+#include <algorithm>
 
 namespace dlp {
 namespace sip {
 
 constexpr int SC_CHUNK = 16;                // blocks of K whose scales are brought in at a time
-constexpr int MAX_STAGES = 12;
-constexpr int NUM_THREADS = 192;            // copies, MMA issue, four warps that sum and store
+constexpr int MAX_STAGES = 8;
 constexpr int MAX_CLUSTER = 8;
 
 struct Shared {
@@ -33,25 +32,24 @@ struct Params {
     int rows, outputs;
     int kblocks;            // of the whole K
     int per_part;           // of a part of K
-    int n_tiles;            // tiles along the columns (of the tile's frame)
-    int y_type, act, stages;
+    int n_tiles;            // tiles of rows of x
+    int y_type, act;
 };
 
-constexpr uint32_t idesc_e4m3(int bn) { return (1u << 4) | (uint32_t(bn >> 3) << 17) | (uint32_t(BM >> 4) << 24); }
+// Warps that sum and store, beside the two that copy and issue: four have a quarter of the tile's rows each; with many columns eight, half of
+// the columns each.
+constexpr int sum_warps_for(int bn) { return bn >= 64 ? 8 : 4; }
+constexpr int threads_for(int bn) { return 64 + 32 * sum_warps_for(bn); }
+// Blocks on an SM, and the ring's stages: what bounds this kernel is the stream of weights, and two blocks with half of the shared memory each
+// fill one another's pauses (48 rows, 4096 -> 24576: one block of eight stages 32.5 us, two of four 25.6).
+constexpr int blocks_for(int bn) { return bn <= 64 ? 2 : 1; }
+constexpr int fixed_for(int bn) { return 2048 + 2 * SC_CHUNK * bn * 4; }                          // alignment slack, barriers, scales
+constexpr int stages_for(int bn) { return std::min(MAX_STAGES, ((SMEM_LIMIT + 1024) / blocks_for(bn) - 1024 - fixed_for(bn)) / ((BM + bn) * BK)); }
 
-__device__ __forceinline__ void tma_load_2d(void *dst, const void *tmap, int x, int y, unsigned long long *bar)
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const void *tmap, int x, int y, uint32_t bar)
 {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                 ::"r"(smem_u32(dst)), "l"(tmap), "r"(x), "r"(y), "r"(smem_u32(bar)) : "memory");
-}
-// the four MMAs of a block of K
-template<int BN> __device__ __forceinline__ void mma_block(uint32_t d, uint64_t a, uint64_t b)
-{
-    #pragma unroll
-    for(int j = 0; j < 4; j++)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                     "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-                     ::"r"(d), "l"(a + 2 * j), "l"(b + 2 * j), "r"(idesc_e4m3(BN)), "r"(j) : "memory");
+                 ::"r"(dst), "l"(tmap), "r"(x), "r"(y), "r"(bar) : "memory");
 }
 __device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank)
 {
@@ -67,31 +65,32 @@ __device__ __forceinline__ void store_out(void *y, long long at, int type, float
     else static_cast<__nv_bfloat16 *>(y)[at] = __float2bfloat16_rn(v);
 }
 
-// SWAP: the tile's rows are rows of w (and its columns rows of x).
-template<int BN, bool SWAP>
-__global__ void __launch_bounds__(NUM_THREADS, 1)
-scaled_ip_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_constant__ CUtensorMap tm_c, const Params q, int *status)
+// A tile is 128 rows of w by BN rows of x.
+template<int BN>
+__global__ void __launch_bounds__(threads_for(BN), blocks_for(BN))
+scaled_ip_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Params q, int *status)
 {
     extern __shared__ unsigned char smem_raw[];
-    constexpr int ACC = BN <= 64 ? 4 : 2;                    // accumulators in tensor memory
-    constexpr int TMEM_COLS = ACC * BN < 32 ? 32 : ACC * BN;
-    constexpr int STAGE_BYTES = (BM + BN) * BK;
-    constexpr int SC = SWAP ? BN : BM;                       // scale products of a block of K
+    constexpr int ACC = 256 * (3 - blocks_for(BN)) / BN > 4 ? 4 : 256 * (3 - blocks_for(BN)) / BN;      // accumulators in tensor memory
+    constexpr int SUM = sum_warps_for(BN), SUM_THREADS = 32 * SUM, COLS = BN * 4 / SUM;      // columns of a summing warp
+    constexpr int TMEM_COLS = ACC * BN;
+    constexpr int S = stages_for(BN), STAGE_BYTES = (BM + BN) * BK;
     unsigned char *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     Shared *sh = reinterpret_cast<Shared *>(smem);
-    float *scale_ring = reinterpret_cast<float *>(smem + 1024);           // two chunks of SC_CHUNK x SC
-    unsigned char *ring = smem + 1024 + 2 * SC_CHUNK * SC * 4;
-    static_assert(sizeof(Shared) <= 1024 && (SC_CHUNK * SC * 8) % 1024 == 0, "ring alignment");
+    float *scale_ring = reinterpret_cast<float *>(smem + 1024);           // two chunks of SC_CHUNK x BN
+    unsigned char *ring = smem + 1024 + 2 * SC_CHUNK * BN * 4;
+    static_assert(sizeof(Shared) <= 1024 && (SC_CHUNK * BN * 8) % 1024 == 0 && S >= 4, "ring");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int S = q.stages;
     const int parts = int(cluster_size()), part = int(cluster_rank());
-    const int tile = int(blockIdx.x) / parts, row_tile = tile / q.n_tiles, col_tile = tile - row_tile * q.n_tiles;
+    const int tile = int(blockIdx.x) / parts, w_tile = tile / q.n_tiles, x_tile = tile - w_tile * q.n_tiles;
     const int kb0 = part * q.per_part, kblocks = max(0, min(q.per_part, q.kblocks - kb0));
     int *abort_flag = &sh->abort_flag;
 
     if(threadIdx.x == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_w) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tm_x) : "memory");
         for(int s = 0; s < S; s++) { mbar_init(&sh->full[s], 1); mbar_init(&sh->empty[s], 1); }
-        for(int a = 0; a < 4; a++) { mbar_init(&sh->acc_full[a], 1); mbar_init(&sh->acc_empty[a], 4); }
+        for(int a = 0; a < ACC; a++) { mbar_init(&sh->acc_full[a], 1); mbar_init(&sh->acc_empty[a], SUM); }
         mbar_init(&sh->drain, 1);
         sh->abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -106,21 +105,24 @@ scaled_ip_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_constant
     const uint32_t tmem_base = *(volatile uint32_t *)&sh->tmem_base;
     pdl_wait();
 
-    constexpr int MINE = SC * SC_CHUNK / 128;                // scale products a summing thread brings in per chunk
-    float acc[BN];
+    constexpr int MINE = BN * SC_CHUNK / SUM_THREADS;                // scale products a summing thread brings in per chunk
+    float acc[COLS];
     #pragma unroll
-    for(int j = 0; j < BN; j++) acc[j] = 0.0f;
-    const int quad = warp & 3, row_in_tile = quad * 32 + lane;
+    for(int j = 0; j < COLS; j++) acc[j] = 0.0f;
+    const int quad = warp & 3, row_in_tile = quad * 32 + lane, col0 = warp >= 6 ? COLS : 0;
 
     if(warp == 0) {
         if(lane == 0) {
+            const uint32_t full0 = smem_u32(&sh->full[0]), empty0 = smem_u32(&sh->empty[0]), ring0 = smem_u32(ring);
+            uint32_t s = 0, phase = 1;
             int kb = 0;
+            #pragma unroll 1
             for(; kb < kblocks; kb++) {
-                const int s = kb % S;
-                if(!mbar_wait(&sh->empty[s], ((kb / S) & 1) ^ 1, abort_flag, status, SIP_EMPTY)) break;
+                if(!mbar_wait(empty0 + 8 * s, phase, abort_flag, status, SIP_EMPTY)) break;
                 mbar_arrive_expect_tx(&sh->full[s], STAGE_BYTES);
-                tma_load_2d(ring + s * STAGE_BYTES, &tm_r, (kb0 + kb) * BK, row_tile * BM, &sh->full[s]);
-                tma_load_2d(ring + s * STAGE_BYTES + BM * BK, &tm_c, (kb0 + kb) * BK, col_tile * BN, &sh->full[s]);
+                tma_load_2d(ring0 + s * STAGE_BYTES, &tm_w, (kb0 + kb) * BK, w_tile * BM, full0 + 8 * s);
+                tma_load_2d(ring0 + s * STAGE_BYTES + BM * BK, &tm_x, (kb0 + kb) * BK, x_tile * BN, full0 + 8 * s);
+                if(++s == S) { s = 0; phase ^= 1; }
             }
             // nothing may still be on its way into shared memory when the block ends
             for(int n = max(0, kb - S); n < kb; n++) {
@@ -131,70 +133,85 @@ scaled_ip_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_constant
                 }
             }
         }
+        __syncwarp();
     }
     else if(warp == 1) {
         if(lane == 0) {
+            constexpr uint32_t IDESC = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(BM >> 4) << 24);     // fp32 sums of e4m3, K-major, M 128
             constexpr uint64_t DESC_HI = uint64_t((1024u >> 4) | (1u << 14) | (2u << 29)) << 32;   // 8-row groups 1024 bytes apart, version 1, SWIZZLE_128B
+            const uint32_t full0 = smem_u32(&sh->full[0]), empty0 = smem_u32(&sh->empty[0]), acc_full0 = smem_u32(&sh->acc_full[0]),
+                           acc_empty0 = smem_u32(&sh->acc_empty[0]), ring0 = ((smem_u32(ring) & 0x3FFFF) >> 4) | (1u << 16);
+            uint32_t s = 0, phase = 0, b = 0, b_phase = 1;
+            #pragma unroll 1
             for(int kb = 0; kb < kblocks; kb++) {
-                const int s = kb % S, b = kb % ACC;
-                if(!mbar_wait(&sh->acc_empty[b], ((kb / ACC) & 1) ^ 1, abort_flag, status, SIP_ACC_EMPTY)) break;
-                if(!mbar_wait(&sh->full[s], (kb / S) & 1, abort_flag, status, SIP_FULL)) break;
+                if(!mbar_wait(acc_empty0 + 8 * b, b_phase, abort_flag, status, SIP_ACC_EMPTY)) break;
+                const uint32_t wd = ring0 + s * (STAGE_BYTES >> 4), xd = wd + (BM * BK >> 4), d = tmem_base + b * BN;
+                if(!mbar_wait(full0 + 8 * s, phase, abort_flag, status, SIP_FULL)) break;
                 tc_fence_after();
-                const uint32_t base = ((smem_u32(ring + s * STAGE_BYTES) & 0x3FFFF) >> 4) | (1u << 16);
-                mma_block<BN>(tmem_base + b * BN, DESC_HI | base, DESC_HI | (base + (BM * BK >> 4)));
-                mma_commit(smem_u32(&sh->empty[s]));
-                mma_commit(smem_u32(&sh->acc_full[b]));
+                #pragma unroll
+                for(int j = 0; j < 4; j++)
+                    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                                 "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                                 ::"r"(d), "l"(DESC_HI | (wd + 2 * j)), "l"(DESC_HI | (xd + 2 * j)), "r"(IDESC), "r"(j) : "memory");
+                mma_commit(empty0 + 8 * s);
+                mma_commit(acc_full0 + 8 * b);
+                if(++s == S) { s = 0; phase ^= 1; }
+                if(++b == ACC) { b = 0; b_phase ^= 1; }
             }
         }
+        __syncwarp();
     }
     else {
         const int t = threadIdx.x - 64;
-        // Products of the scales for the chunk of blocks of K at kb, [block][row of the tile, or column]; zero beyond the matrices.
+        const uint32_t acc_full0 = smem_u32(&sh->acc_full[0]), acc_empty0 = smem_u32(&sh->acc_empty[0]);
+        // Products of the scales for the chunk of blocks of K at kb, [block][row of x]; zero beyond the matrices.
         float next[MINE];
         auto fetch = [&](int kb) {
             #pragma unroll
             for(int i = 0; i < MINE; i++) {
-                const int at = i * 128 + t, b = kb0 + kb + at / SC, j = at % SC;
-                const int r = SWAP ? col_tile * BN + j : row_tile * BM + j;
-                const int o = SWAP ? row_tile : col_tile * BN / SCALE_BLOCK;
-                next[i] = kb + at / SC < kblocks && r < q.rows ? ld_plain(q.x_scales + b * q.x_scale_stride + r) * ld_plain(q.w_scales + o * q.w_scale_stride + b)
-                                                               : 0.0f;
+                const int at = i * SUM_THREADS + t, k = kb + at / BN, r = x_tile * BN + at % BN;
+                next[i] = k < kblocks && r < q.rows ? ld_plain(q.x_scales + (kb0 + k) * q.x_scale_stride + r) * ld_plain(q.w_scales + w_tile * q.w_scale_stride + kb0 + k)
+                                                    : 0.0f;
             }
         };
-        static_assert(SWAP || BN <= SCALE_BLOCK, "one scale of w per tile");
         if(kblocks > 0) fetch(0);
-        bool live = true;
+        uint32_t b = 0, b_phase = 0;
+        #pragma unroll 1
         for(int kb = 0; kb < kblocks; kb++) {
-            const int in = kb % SC_CHUNK, b = kb % ACC;
-            float *sc = scale_ring + (kb / SC_CHUNK & 1) * SC_CHUNK * SC;
+            const int in = kb % SC_CHUNK;
+            const float *sc = scale_ring + ((kb / SC_CHUNK & 1) * SC_CHUNK + in) * BN + col0;
             if(in == 0) {
                 #pragma unroll
-                for(int i = 0; i < MINE; i++) sc[i * 128 + t] = next[i];
-                asm volatile("bar.sync 1, 128;" ::: "memory");
+                for(int i = 0; i < MINE; i++) scale_ring[(kb / SC_CHUNK & 1) * SC_CHUNK * BN + i * SUM_THREADS + t] = next[i];
+                asm volatile("bar.sync 1, %0;" ::"n"(SUM_THREADS) : "memory");
                 if(kb + SC_CHUNK < kblocks) fetch(kb + SC_CHUNK);
             }
-            if(live && !warp_wait(&sh->acc_full[b], (kb / ACC) & 1, abort_flag, status, SIP_ACC_FULL, lane)) live = false;
-            if(!live) continue;                              // (the barriers above are met on every path)
+            // (no vote: should the wait give up, the others do so at once, and what is read means nothing)
+            if(lane == 0) mbar_wait(acc_full0 + 8 * b, b_phase, abort_flag, status, SIP_ACC_FULL);
+            __syncwarp();
             tc_fence_after();
-            const uint32_t taddr = tmem_base + (uint32_t(quad * 32) << 16) + b * BN;
-            const float mine = SWAP ? 0.0f : sc[in * SC + row_in_tile];
+            const uint32_t taddr = tmem_base + (uint32_t(quad * 32) << 16) + b * BN + col0;
+            constexpr int W = COLS < 32 ? 16 : 32;
             #pragma unroll
-            for(int g = 0; g < BN / 16; g++) {
-                uint32_t v[16];
-                tmem_ld16(taddr + g * 16, v);
+            for(int g = 0; g < COLS / W; g++) {
+                uint32_t v[W];
+                tmem_ld(taddr + g * W, v);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                if(g + 1 == COLS / W) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if(lane == 0) mbar_arrive(acc_empty0 + 8 * b);
+                }
                 #pragma unroll
-                for(int j = 0; j < 16; j += 4) {
-                    const float4 f = SWAP ? *reinterpret_cast<const float4 *>(sc + in * SC + g * 16 + j) : make_float4(mine, mine, mine, mine);
-                    acc[g * 16 + j] += __uint_as_float(v[j]) * f.x;
-                    acc[g * 16 + j + 1] += __uint_as_float(v[j + 1]) * f.y;
-                    acc[g * 16 + j + 2] += __uint_as_float(v[j + 2]) * f.z;
-                    acc[g * 16 + j + 3] += __uint_as_float(v[j + 3]) * f.w;
+                for(int j = 0; j < W; j += 4) {
+                    const float4 f = *reinterpret_cast<const float4 *>(sc + g * W + j);
+                    acc[g * W + j] += __uint_as_float(v[j]) * f.x;
+                    acc[g * W + j + 1] += __uint_as_float(v[j + 1]) * f.y;
+                    acc[g * W + j + 2] += __uint_as_float(v[j + 2]) * f.z;
+                    acc[g * W + j + 3] += __uint_as_float(v[j + 3]) * f.w;
                 }
             }
-            tc_fence_before();
-            __syncwarp();
-            if(lane == 0) mbar_arrive(&sh->acc_empty[b]);
+            if(++b == ACC) { b = 0; b_phase ^= 1; }
         }
     }
 
@@ -219,51 +236,43 @@ scaled_ip_kernel(const __grid_constant__ CUtensorMap tm_r, const __grid_constant
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
     }
 
-    // ---- sum over the parts of K, bias, activation, store
+    // ---- sum over the parts of K, bias, activation, store: a warp stores 32 outputs of a row of x
+    const int o = w_tile * BM + row_in_tile, rows = min(BN, q.rows - x_tile * BN);
     if(parts > 1) {
-        // a part's sums as [column][row of the tile], where its operands were
+        // a part's sums as [row of x][row of w], where its operands were
         float *partial = reinterpret_cast<float *>(ring);
         if(warp >= 2) {
             #pragma unroll
-            for(int j = 0; j < BN; j++) partial[j * BM + row_in_tile] = acc[j];
+            for(int j = 0; j < COLS; j++)
+                if(col0 + j < rows) partial[(col0 + j) * BM + row_in_tile] = acc[j];
         }
-        __syncthreads();
         cluster_sync();
         if(warp >= 2) {
-            // part p of the cluster finishes columns p, p + parts, ...
-            const uint32_t base = smem_u32(partial);
-            const int o = row_tile * BM + row_in_tile;
+            // part p of the cluster finishes rows p, p + parts, ...
+            const uint32_t base = smem_u32(partial) + row_in_tile * 4;
             const float bias = q.bias && o < q.outputs ? ld_plain(q.bias + o) : 0.0f;
-            for(int j = part; j < BN && col_tile * BN + j < q.rows; j += parts) {
-                float sum = 0.0f;
-                for(int p = 0; p < parts; p++) sum += ld_cluster(base + (j * BM + row_in_tile) * 4, p);
-                if(o < q.outputs) store_out(q.y, (long long)(col_tile * BN + j) * q.y_stride + o, q.y_type, apply_act(sum + bias, q.act));
+            #pragma unroll 1
+            for(int j = part + (warp >= 6 ? parts : 0); j < rows; j += parts * (SUM / 4)) {
+                float v[MAX_CLUSTER];
+                #pragma unroll
+                for(int p = 0; p < MAX_CLUSTER; p++) v[p] = p < parts ? ld_cluster(base + j * (BM * 4), p) : 0.0f;
+                float sum = v[0];
+                #pragma unroll
+                for(int p = 1; p < MAX_CLUSTER; p++) sum += v[p];
+                if(o < q.outputs) store_out(q.y, (long long)(x_tile * BN + j) * q.y_stride + o, q.y_type, apply_act(sum + bias, q.act));
             }
         }
-        __syncthreads();
         cluster_sync();                                      // nobody leaves while its sums are being read
     }
-    else if(warp >= 2) {
-        if(SWAP) {
-            const int o = row_tile * BM + row_in_tile;
-            const float bias = q.bias && o < q.outputs ? ld_plain(q.bias + o) : 0.0f;
-            if(o < q.outputs) {
-                #pragma unroll
-                for(int j = 0; j < BN; j++)
-                    if(col_tile * BN + j < q.rows)
-                        store_out(q.y, (long long)(col_tile * BN + j) * q.y_stride + o, q.y_type, apply_act(acc[j] + bias, q.act));
+    else if(warp >= 2 && o < q.outputs) {
+        const float bias = q.bias ? ld_plain(q.bias + o) : 0.0f;
+        #pragma unroll
+        for(int j = 0; j < COLS; j++)
+            if(col0 + j < rows) {
+                float v = acc[j] + bias;
+                if(q.act != DLP_ACT_IDENTITY) v = apply_act(v, q.act);
+                store_out(q.y, (long long)(x_tile * BN + col0 + j) * q.y_stride + o, q.y_type, v);
             }
-        }
-        else {
-            const int r = row_tile * BM + row_in_tile;
-            if(r < q.rows) {
-                #pragma unroll
-                for(int j = 0; j < BN; j++) {
-                    const int o = col_tile * BN + j;
-                    if(o < q.outputs) store_out(q.y, r * q.y_stride + o, q.y_type, apply_act(acc[j] + (q.bias ? ld_plain(q.bias + o) : 0.0f), q.act));
-                }
-            }
-        }
     }
 }
 
@@ -292,7 +301,7 @@ static dlp_status encode_2d(CUtensorMap &map, CUtensorMapDataType type, const vo
     cuuint64_t dims[2] = { cuuint64_t(cols), cuuint64_t(rows) }, strides[1] = { cuuint64_t(stride_bytes) };
     cuuint32_t box[2] = { cuuint32_t(box_cols), cuuint32_t(box_rows) }, elem[2] = { 1, 1 };
     const CUresult r = enc(&map, type, 2, const_cast<void *>(p), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                           CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if(r != CUDA_SUCCESS) return fail(DLP_CUDA_ERROR, "cuTensorMapEncodeTiled failed with code " + std::to_string(int(r)));
     return DLP_OK;
 }
@@ -308,27 +317,27 @@ dlp_status encode_result(CUtensorMap &map, const Problem &p)
     return encode_2d(map, type, p.y, p.outputs, p.rows, p.y_stride * size, 128 / size, 32);
 }
 
-template<int BN, bool SWAP>
-static dlp_status launch(const Problem &p, int parts, cudaStream_t stream)
+template<int BN> static dlp_status launch(const Problem &p, cudaStream_t stream)
 {
-    dlp_status st = allow_shared<scaled_ip_kernel<BN, SWAP>>(SMEM_LIMIT);
+    dlp_status st = allow_shared<scaled_ip_few_kernel<BN>>(SMEM_LIMIT);
     if(st != DLP_OK) return st;
     int *status = device_status_word();
     if(!status) return fail(DLP_CUDA_ERROR, "cannot resolve the device status word");
-    Params q = { p.x_scales, p.w_scales, p.bias, p.y, p.x_scale_stride, p.w_scale_stride, p.y_stride, p.rows, p.outputs, p.kblocks,
-                 ceil_div(p.kblocks, parts), 0, p.y_type, p.act, 0 };
+    const int w_tiles = ceil_div(p.outputs, BM), x_tiles = ceil_div(p.rows, BN), slots = sm_count() * blocks_for(BN);
+    // parts of K until the places on the SMs are taken
+    int parts = 1;
+    while(parts < MAX_CLUSTER && parts * 2 <= p.kblocks && (long long)w_tiles * x_tiles * parts * 2 <= slots) parts *= 2;
+    const Params q = { p.x_scales, p.w_scales, p.bias, p.y, p.x_scale_stride, p.w_scale_stride, p.y_stride, p.rows, p.outputs, p.kblocks,
+                       ceil_div(p.kblocks, parts), x_tiles, p.y_type, p.act };
     CUtensorMap mx, mw;
-    st = encode_operand(mx, p.x, p.x_stride, p.rows, p.inputs, SWAP ? BN : BM);
-    if(st == DLP_OK) st = encode_operand(mw, p.w, p.w_stride, p.outputs, p.inputs, SWAP ? BM : BN);
+    st = encode_operand(mx, p.x, p.x_stride, p.rows, p.inputs, BN);
+    if(st == DLP_OK) st = encode_operand(mw, p.w, p.w_stride, p.outputs, p.inputs, BM);
     if(st != DLP_OK) return st;
-    const int fixed = 2048 + 2 * SC_CHUNK * (SWAP ? BN : BM) * 4, stage = (BM + BN) * BK;
-    q.stages = std::min(MAX_STAGES, (SMEM_LIMIT - fixed) / stage);
-    q.n_tiles = SWAP ? ceil_div(q.rows, BN) : ceil_div(q.outputs, BN);
-    const long long blocks = (long long)q.n_tiles * ceil_div(SWAP ? q.outputs : q.rows, BM) * parts;
+    const long long blocks = (long long)w_tiles * x_tiles * parts;
     DLP_REQUIRE(blocks < (1ll << 31), "too many tiles");
-    const int smem = fixed + q.stages * stage;
-    DLP_LAUNCH_PDL(launch_pdl_cluster(few_items(blocks), parts, scaled_ip_kernel<BN, SWAP>, unsigned(blocks), NUM_THREADS, smem, stream, SWAP ? mw : mx,
-                                      SWAP ? mx : mw, q, status), "scaled_ip_kernel");
+    constexpr int smem = fixed_for(BN) + stages_for(BN) * (BM + BN) * BK;
+    DLP_LAUNCH_PDL(launch_pdl_cluster(blocks <= slots, parts, scaled_ip_few_kernel<BN>, unsigned(blocks), threads_for(BN), smem, stream, mw, mx, q, status),
+                   "scaled_ip_few_kernel");
     return DLP_OK;
 }
 
@@ -339,10 +348,10 @@ using namespace dlp;
 
 extern "C" {
 
-dlp_status dlp_scaled_ip_fwd(const void *x, long long x_stride, const float *x_scales, long long x_scale_stride, const void *w,
-                             long long w_stride, const float *w_scales, long long w_scale_stride, const float *bias, void *y,
-                             long long y_stride, int y_type, int activation, int rows, int inputs, int outputs, void *stream)
+dlp_status dlp_scaled_ip_fwd(const dlp_scaled_ip_args *args, void *stream)
 {
+    DLP_REQUIRE(args != nullptr, "null arguments");
+    const auto [x, x_scales, w, w_scales, bias, y, x_stride, x_scale_stride, w_stride, w_scale_stride, y_stride, rows, inputs, outputs, y_type, activation] = *args;
     DLP_REQUIRE(rows >= 0 && inputs > 0 && outputs > 0, "bad shape");
     DLP_REQUIRE(inputs <= (1 << 30) && outputs <= (1 << 30) && rows <= (1 << 30), "too large");
     DLP_REQUIRE(is_real_type(y_type), "the result's type must be fp32, fp16 or bf16");
@@ -361,13 +370,10 @@ dlp_status dlp_scaled_ip_fwd(const void *x, long long x_stride, const float *x_s
                              kblocks, y_type, activation };
     cudaStream_t s = (cudaStream_t)stream;
     if(rows > 128) return sip::launch_pair(p, s);
-    // parts of K until every SM has a tile
-    int parts = 1;
-    while(parts < sip::MAX_CLUSTER && parts * 2 <= kblocks && oblocks * parts * 2 <= sm_count()) parts *= 2;
-    if(rows <= 16) return sip::launch<16, true>(p, parts, s);
-    if(rows <= 32) return sip::launch<32, true>(p, parts, s);
-    if(rows <= 64) return sip::launch<64, true>(p, parts, s);
-    return sip::launch<128, true>(p, parts, s);
+    if(rows <= 16) return sip::launch<16>(p, s);
+    if(rows <= 32) return sip::launch<32>(p, s);
+    if(rows <= 64) return sip::launch<64>(p, s);
+    return sip::launch<128>(p, s);
 }
 
 } // extern "C"

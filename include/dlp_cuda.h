@@ -288,39 +288,68 @@ enum { DLP_GATE_NONE = 0, DLP_GATE_SILU = 1, DLP_GATE_GELU = 2 };
 
 /* Root-mean-square norm of each row, with a residual added before it:
  *     h = x + residual;   total = h;   y = h / sqrt(mean(h^2) + eps) * weight.
- * x, residual, total and weight are of `type` (fp32, fp16 or bf16), y of y_type: any of these, or e4m3 in blocks of one row, then with
- * scales.  h is fp32 throughout; only what is stored is rounded.  residual may be NULL; total may be NULL, or be x or residual itself
- * (the same address and stride). */
-DLP_API dlp_status dlp_rms_norm_fwd(const void *x, long long x_stride, const void *residual, long long residual_stride, void *total,
-                                    long long total_stride, const void *weight, int type, void *y, long long y_stride, int y_type,
-                                    float *scales, long long scale_stride, int rows, int cols, float eps, void *stream);
+ * h is fp32 throughout; only what is stored is rounded. */
+typedef struct dlp_rms_norm_args {
+    const void *x;              /* [rows, cols] of `type` (fp32, fp16 or bf16) */
+    const void *residual;       /* the same, or NULL */
+    const void *weight;         /* [cols] of `type` */
+    void *total;                /* [rows, cols] of `type`, or NULL; may be x or residual itself (the same address and stride) */
+    void *y;                    /* [rows, cols] of y_type: fp32, fp16, bf16, or e4m3 in blocks of one row */
+    float *scales;              /* of an e4m3 y; NULL otherwise */
+    long long x_stride, residual_stride, total_stride, y_stride, scale_stride;
+    int rows, cols, type, y_type;
+    float eps;                  /* positive */
+} dlp_rms_norm_args;
+DLP_API dlp_status dlp_rms_norm_fwd(const dlp_rms_norm_args *args, void *stream);
 
 /* 8-bit form of x [rows, cols] (gate DLP_GATE_NONE), or of act(a) * b where x [rows, 2 * cols] holds a in its first cols columns and b in the
- * others: silu(a) = a / (1 + exp(-a)), gelu(a) = a / 2 * (1 + tanh(sqrt(2 / pi) * (a + 0.044715 a^3))), in fp32.  block_rows: 1, or 128 for
- * weights (without a gate). */
-DLP_API dlp_status dlp_quantize_fwd(const void *x, long long x_stride, int type, int gate, void *q, long long q_stride, float *scales,
-                                    long long scale_stride, int block_rows, int rows, int cols, void *stream);
+ * others: silu(a) = a / (1 + exp(-a)), gelu(a) = a / 2 * (1 + tanh(sqrt(2 / pi) * (a + 0.044715 a^3))), in fp32. */
+typedef struct dlp_quantize_args {
+    const void *x;              /* of `type` (fp32, fp16 or bf16) */
+    void *q;                    /* [rows, cols], e4m3 */
+    float *scales;
+    long long x_stride, q_stride, scale_stride;
+    int rows, cols, type, gate; /* gate: DLP_GATE_* */
+    int block_rows;             /* 1, or 128 for weights (without a gate) */
+} dlp_quantize_args;
+DLP_API dlp_status dlp_quantize_fwd(const dlp_quantize_args *args, void *stream);
 
 /* InnerProduct of 8-bit operands, on the tensor cores:
- *     y[rows, outputs] = act(x[rows, inputs] * w[outputs, inputs]^T + bias[outputs])
- * x in blocks of one row, w in blocks of 128 x 128.  Products are summed in fp32; y is of y_type (fp32, fp16 or bf16), bias is fp32 or NULL.
- * x and w are 16-byte aligned, their row strides multiples of 16.  The result does not depend on timing. */
-DLP_API dlp_status dlp_scaled_ip_fwd(const void *x, long long x_stride, const float *x_scales, long long x_scale_stride, const void *w,
-                                     long long w_stride, const float *w_scales, long long w_scale_stride, const float *bias, void *y,
-                                     long long y_stride, int y_type, int activation, int rows, int inputs, int outputs, void *stream);
+ *     y[rows, outputs] = act(x[rows, inputs] * w[outputs, inputs]^T + bias[outputs]).
+ * Products are summed in fp32.  The result does not depend on timing. */
+typedef struct dlp_scaled_ip_args {
+    const void *x;              /* [rows, inputs], e4m3 in blocks of one row; 16-byte aligned, x_stride a multiple of 16 */
+    const float *x_scales;
+    const void *w;              /* [outputs, inputs], e4m3 in blocks of 128 x 128; 16-byte aligned, w_stride a multiple of 16 */
+    const float *w_scales;
+    const float *bias;          /* [outputs] or NULL */
+    void *y;                    /* [rows, outputs] of y_type: fp32, fp16 or bf16 */
+    long long x_stride, x_scale_stride, w_stride, w_scale_stride, y_stride;
+    int rows, inputs, outputs, y_type;
+    int activation;             /* DLP_ACT_* */
+} dlp_scaled_ip_args;
+DLP_API dlp_status dlp_scaled_ip_fwd(const dlp_scaled_ip_args *args, void *stream);
 
-/* Draws a class from each row of logits (fp32, fp16 or bf16) with the row's random number u, 0 <= u < 1.
+/* Draws a class from each row of logits with the row's random number u, 0 <= u < 1.
  * With a row's classes in the order of falling logits, equal ones in the order of their index, and masses exp((logit - largest) / temperature):
  * top_k keeps the first k; top_p keeps of these the shortest prefix that has at least p of their mass (never less than one); min_p keeps of
  * these the ones whose mass is at least m times the largest one's.  The class drawn is the first one, by index, at which the running mass of
  * the kept ones exceeds u times their whole mass.
- * temperature, top_k, top_p, min_p: one value for each row, or NULL (1, and all kept).  A temperature that is not positive means the largest
- * logit, the lowest index of equal ones; k <= 0 or >= classes, p >= 1 and m <= 0 keep everything; m above 1 counts as 1.  A logit of -inf or
- * NaN is never drawn; a row of nothing else gives -1.  Logits of +inf share the whole mass.  Masses are summed as whole numbers of at least 41
- * bits, so the result depends neither on timing nor on the order of sums. */
+ * A temperature that is not positive means the largest logit, the lowest index of equal ones; k <= 0 or >= classes, p >= 1 and m <= 0 keep
+ * everything; m above 1 counts as 1.  A logit of -inf or NaN is never drawn; a row of nothing else gives -1.  Logits of +inf share the whole
+ * mass.  Masses are summed as whole numbers of at least 41 bits, so the result depends neither on timing nor on the order of sums. */
 #define DLP_SAMPLE_MAX_CLASSES (1 << 22)
-DLP_API dlp_status dlp_sample_fwd(const void *logits, long long stride, int type, int rows, int classes, const float *temperature, const int *top_k,
-                                  const float *top_p, const float *min_p, const float *u, int *tokens, void *stream);
+typedef struct dlp_sample_args {
+    const void *logits;         /* [rows, classes] of `type` (fp32, fp16 or bf16) */
+    const float *temperature;   /* one value for each row, or NULL: 1 */
+    const int *top_k;           /* the same, or NULL: all are kept */
+    const float *top_p, *min_p;
+    const float *u;             /* [rows] */
+    int *tokens;                /* [rows] */
+    long long stride;
+    int rows, classes, type;
+} dlp_sample_args;
+DLP_API dlp_status dlp_sample_fwd(const dlp_sample_args *args, void *stream);
 
 #ifdef __cplusplus
 }
