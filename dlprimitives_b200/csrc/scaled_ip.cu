@@ -111,8 +111,10 @@ scaled_ip_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
     for(int j = 0; j < COLS; j++) acc[j] = 0.0f;
     const int quad = warp & 3, row_in_tile = quad * 32 + lane, col0 = warp >= 6 ? COLS : 0;
 
+    // (One elected thread copies and one issues; the compiler then knows that it is one, and takes the operands of a tcgen05.mma as they are.  Chosen by
+    // its lane number it brings them together for each instruction: 370 instead of 170 cycles for four of them and two commits.)
     if(warp == 0) {
-        if(lane == 0) {
+        if(elect_one()) {
             const uint32_t full0 = smem_u32(&sh->full[0]), empty0 = smem_u32(&sh->empty[0]), ring0 = smem_u32(ring);
             uint32_t s = 0, phase = 1;
             int kb = 0;
@@ -136,7 +138,7 @@ scaled_ip_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
         __syncwarp();
     }
     else if(warp == 1) {
-        if(lane == 0) {
+        if(elect_one()) {
             constexpr uint32_t IDESC = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(BM >> 4) << 24);     // fp32 sums of e4m3, K-major, M 128
             constexpr uint64_t DESC_HI = uint64_t((1024u >> 4) | (1u << 14) | (2u << 29)) << 32;   // 8-row groups 1024 bytes apart, version 1, SWIZZLE_128B
             const uint32_t full0 = smem_u32(&sh->full[0]), empty0 = smem_u32(&sh->empty[0]), acc_full0 = smem_u32(&sh->acc_full[0]),
@@ -220,7 +222,7 @@ scaled_ip_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
     __syncthreads();
     if(*(volatile int *)abort_flag) {
         // a wait gave up: let the MMAs already issued retire (bounded) before tensor memory goes away
-        if(warp == 1 && lane == 0) {
+        if(warp == 1 && elect_one()) {
             mma_commit(smem_u32(&sh->drain));
             const long long t0 = global_ns();
             while(!mbar_try_wait(&sh->drain, 0)) {
@@ -335,7 +337,8 @@ template<int BN> static dlp_status launch(const Problem &p, cudaStream_t stream)
     if(st != DLP_OK) return st;
     const long long blocks = (long long)w_tiles * x_tiles * parts;
     DLP_REQUIRE(blocks < (1ll << 31), "too many tiles");
-    constexpr int smem = fixed_for(BN) + stages_for(BN) * (BM + BN) * BK;
+    // (a short part of K needs no more stages than it has blocks; the places left let the next kernel's blocks be set up early)
+    const int smem = fixed_for(BN) + std::max(std::min(stages_for(BN), q.per_part), ceil_div(BN * BM * 4, (BM + BN) * BK)) * (BM + BN) * BK;
     DLP_LAUNCH_PDL(launch_pdl_cluster(blocks <= slots, parts, scaled_ip_few_kernel<BN>, unsigned(blocks), threads_for(BN), smem, stream, mw, mx, q, status),
                    "scaled_ip_few_kernel");
     return DLP_OK;

@@ -116,58 +116,65 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
 
     if(warp < WARP_SUM0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ISSUE));
-        if(warp == WARP_COPY && lane == 0) {
-            uint32_t s = 0, phase = 1, count = 0;
-            bool live = true;
-            const uint32_t full0 = place_in(smem_u32(&sh->full[0]), 0), empty0 = smem_u32(&sh->empty[0]);
-            for(int t = first; t < tiles && live; t += step) {
-                const Tile w = tile_at(t, q);
-                const int x_row = w.row * 2 * BM + int(rank) * BM, w_row = w.col * BN + int(rank) * (BN / 2);
-                #pragma unroll 1
-                for(int kb = 0; kb < kblocks; kb++) {
-                    if(!mbar_wait(empty0 + 8 * s, phase, abort_flag, status, SIP_EMPTY)) { live = false; break; }
-                    const uint32_t slot = ring0 + s * STAGE_BYTES, bar = full0 + 8 * s;
-                    if(rank == 0) mbar_arrive_expect_tx(&sh->full[s], 2 * STAGE_BYTES);
-                    tma_load_pair(slot, &tm_x, kb * BK, x_row, bar);
-                    tma_load_pair(slot + X_BYTES, &tm_w, kb * BK, w_row, bar);
-                    count++;
-                    if(++s == S) { s = 0; phase ^= 1; }
-                }
-            }
-            // nothing may still be on its way into shared memory when the blocks end (the other block waits for this one below)
-            if(rank == 0)
-                for(uint32_t n = count > uint32_t(S) ? count - S : 0; n < count; n++) {
-                    const long long t0 = global_ns();
-                    while(!mbar_try_wait(&sh->full[n % S], (n / S) & 1)) {
-                        __nanosleep(256);
-                        if(global_ns() - t0 > WAIT_LIMIT_NS) { atomicCAS(status, 0, SIP_DRAIN); break; }
+        // (elected threads: see scaled_ip_few_kernel)
+        if(warp == WARP_COPY) {
+            if(elect_one()) {
+                uint32_t s = 0, phase = 1, count = 0;
+                bool live = true;
+                const uint32_t full0 = place_in(smem_u32(&sh->full[0]), 0), empty0 = smem_u32(&sh->empty[0]);
+                for(int t = first; t < tiles && live; t += step) {
+                    const Tile w = tile_at(t, q);
+                    const int x_row = w.row * 2 * BM + int(rank) * BM, w_row = w.col * BN + int(rank) * (BN / 2);
+                    #pragma unroll 1
+                    for(int kb = 0; kb < kblocks; kb++) {
+                        if(!mbar_wait(empty0 + 8 * s, phase, abort_flag, status, SIP_EMPTY)) { live = false; break; }
+                        const uint32_t slot = ring0 + s * STAGE_BYTES, bar = full0 + 8 * s;
+                        if(rank == 0) mbar_arrive_expect_tx(&sh->full[s], 2 * STAGE_BYTES);
+                        tma_load_pair(slot, &tm_x, kb * BK, x_row, bar);
+                        tma_load_pair(slot + X_BYTES, &tm_w, kb * BK, w_row, bar);
+                        count++;
+                        if(++s == S) { s = 0; phase ^= 1; }
                     }
                 }
-        }
-        else if(warp == WARP_MMA && lane == 0 && rank == 0) {
-            constexpr uint32_t IDESC = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(2 * BM >> 4) << 24);     // fp32 sums of e4m3, K-major, M 256
-            constexpr uint64_t DESC_HI = uint64_t((1024u >> 4) | (1u << 14) | (2u << 29)) << 32;   // 8-row groups 1024 bytes apart, version 1, SWIZZLE_128B
-            const uint32_t ring = ((ring0 & 0x3FFFF) >> 4) | (1u << 16);
-            const uint32_t full0 = smem_u32(&sh->full[0]), empty0 = smem_u32(&sh->empty[0]), acc_full0 = smem_u32(&sh->acc_full[0]), acc_empty0 = smem_u32(&sh->acc_empty[0]);
-            uint32_t s = 0, phase = 0, b = 0, b_phase = 1;
-            const long long total = (long long)((tiles - first + step - 1) / step) * kblocks;
-            #pragma unroll 1
-            for(long long it = 0; it < total; it++) {
-                // (the operands have been there for a while; the accumulator is what is waited for)
-                if(!mbar_wait(full0 + 8 * s, phase, abort_flag, status, SIP_FULL)) break;
-                const uint32_t xd = ring + s * (STAGE_BYTES >> 4), wd = xd + (X_BYTES >> 4), d = tmem_base + b * BN;
-                if(!mbar_wait(acc_empty0 + 8 * b, b_phase, abort_flag, status, SIP_ACC_EMPTY)) break;
-                tc_fence_after();
-                #pragma unroll
-                for(int j = 0; j < 4; j++)
-                    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                                 "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-                                 ::"r"(d), "l"(DESC_HI | (xd + 2 * j)), "l"(DESC_HI | (wd + 2 * j)), "r"(IDESC), "r"(j) : "memory");
-                commit_pair(acc_full0 + 8 * b);
-                commit_pair(empty0 + 8 * s);
-                if(++s == S) { s = 0; phase ^= 1; }
-                if(++b == ACC) { b = 0; b_phase ^= 1; }
+                // nothing may still be on its way into shared memory when the blocks end (the other block waits for this one below)
+                if(rank == 0)
+                    for(uint32_t n = count > uint32_t(S) ? count - S : 0; n < count; n++) {
+                        const long long t0 = global_ns();
+                        while(!mbar_try_wait(&sh->full[n % S], (n / S) & 1)) {
+                            __nanosleep(256);
+                            if(global_ns() - t0 > WAIT_LIMIT_NS) { atomicCAS(status, 0, SIP_DRAIN); break; }
+                        }
+                    }
             }
+            __syncwarp();
+        }
+        else if(warp == WARP_MMA) {
+            if(rank == 0 && elect_one()) {
+                constexpr uint32_t IDESC = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(2 * BM >> 4) << 24);     // fp32 sums of e4m3, K-major, M 256
+                constexpr uint64_t DESC_HI = uint64_t((1024u >> 4) | (1u << 14) | (2u << 29)) << 32;   // 8-row groups 1024 bytes apart, version 1, SWIZZLE_128B
+                const uint32_t ring = ((ring0 & 0x3FFFF) >> 4) | (1u << 16);
+                const uint32_t full0 = smem_u32(&sh->full[0]), empty0 = smem_u32(&sh->empty[0]), acc_full0 = smem_u32(&sh->acc_full[0]), acc_empty0 = smem_u32(&sh->acc_empty[0]);
+                uint32_t s = 0, phase = 0, b = 0, b_phase = 1;
+                const long long total = (long long)((tiles - first + step - 1) / step) * kblocks;
+                #pragma unroll 1
+                for(long long it = 0; it < total; it++) {
+                    // (the operands have been there for a while; the accumulator is what is waited for)
+                    if(!mbar_wait(full0 + 8 * s, phase, abort_flag, status, SIP_FULL)) break;
+                    const uint32_t xd = ring + s * (STAGE_BYTES >> 4), wd = xd + (X_BYTES >> 4), d = tmem_base + b * BN;
+                    if(!mbar_wait(acc_empty0 + 8 * b, b_phase, abort_flag, status, SIP_ACC_EMPTY)) break;
+                    tc_fence_after();
+                    #pragma unroll
+                    for(int j = 0; j < 4; j++)
+                        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                                     "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                                     ::"r"(d), "l"(DESC_HI | (xd + 2 * j)), "l"(DESC_HI | (wd + 2 * j)), "r"(IDESC), "r"(j) : "memory");
+                    commit_pair(acc_full0 + 8 * b);
+                    commit_pair(empty0 + 8 * s);
+                    if(++s == S) { s = 0; phase ^= 1; }
+                    if(++b == ACC) { b = 0; b_phase ^= 1; }
+                }
+            }
+            __syncwarp();
         }
         else if(warp >= WARP_SCALE0) {
             // products of the two scales, a chunk of blocks of K at a time; a lane has two of the tile's rows
@@ -374,7 +381,7 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
     __syncthreads();
     if(rank == 0 && *(volatile int *)abort_flag) {
         // a wait gave up: let the MMAs already issued retire (bounded) before tensor memory goes away
-        if(warp == WARP_MMA && lane == 0) {
+        if(warp == WARP_MMA && elect_one()) {
             asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(&sh->drain)) : "memory");
             const long long t0 = global_ns();
             while(!mbar_try_wait(&sh->drain, 0)) {
