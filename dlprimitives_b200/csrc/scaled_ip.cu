@@ -167,13 +167,14 @@ scaled_ip_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
         const int t = threadIdx.x - 64;
         const uint32_t acc_full0 = smem_u32(&sh->acc_full[0]), acc_empty0 = smem_u32(&sh->acc_empty[0]);
         // Products of the scales for the chunk of blocks of K at kb, [block][row of x]; zero beyond the matrices.
-        float next[MINE];
+        float next_x[MINE], next_w[MINE];
         auto fetch = [&](int kb) {
             #pragma unroll
             for(int i = 0; i < MINE; i++) {
                 const int at = i * SUM_THREADS + t, k = kb + at / BN, r = x_tile * BN + at % BN;
-                next[i] = k < kblocks && r < q.rows ? ld_plain(q.x_scales + (kb0 + k) * q.x_scale_stride + r) * ld_plain(q.w_scales + w_tile * q.w_scale_stride + kb0 + k)
-                                                    : 0.0f;
+                const bool there = k < kblocks && r < q.rows;
+                next_x[i] = there ? ld_plain(q.x_scales + (kb0 + k) * q.x_scale_stride + r) : 0.0f;
+                next_w[i] = there ? ld_plain(q.w_scales + w_tile * q.w_scale_stride + kb0 + k) : 0.0f;
             }
         };
         if(kblocks > 0) fetch(0);
@@ -184,7 +185,7 @@ scaled_ip_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
             const float *sc = scale_ring + ((kb / SC_CHUNK & 1) * SC_CHUNK + in) * BN + col0;
             if(in == 0) {
                 #pragma unroll
-                for(int i = 0; i < MINE; i++) scale_ring[(kb / SC_CHUNK & 1) * SC_CHUNK * BN + i * SUM_THREADS + t] = next[i];
+                for(int i = 0; i < MINE; i++) scale_ring[(kb / SC_CHUNK & 1) * SC_CHUNK * BN + i * SUM_THREADS + t] = next_x[i] * next_w[i];
                 asm volatile("bar.sync 1, %0;" ::"n"(SUM_THREADS) : "memory");
                 if(kb + SC_CHUNK < kblocks) fetch(kb + SC_CHUNK);
             }
@@ -193,7 +194,7 @@ scaled_ip_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
             __syncwarp();
             tc_fence_after();
             const uint32_t taddr = tmem_base + (uint32_t(quad * 32) << 16) + b * BN + col0;
-            constexpr int W = COLS < 32 ? 16 : 32;
+            constexpr int W = BN == 128 ? 32 : 16;
             #pragma unroll
             for(int g = 0; g < COLS / W; g++) {
                 uint32_t v[W];
@@ -238,44 +239,41 @@ scaled_ip_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS) : "memory");
     }
 
-    // ---- sum over the parts of K, bias, activation, store: a warp stores 32 outputs of a row of x
+    // ---- sum over the parts of K, bias, activation, store: a warp stores 32 outputs of a row of x.  The sums pass through shared memory in any case, where
+    // the operands were: from there a short loop takes them row by row (unrolled over registers, with three types and five activations, the code was
+    // longer than the rest of the kernel, and fetching it took 6 us).
     const int o = w_tile * BM + row_in_tile, rows = min(BN, q.rows - x_tile * BN);
-    if(parts > 1) {
-        // a part's sums as [row of x][row of w], where its operands were
-        float *partial = reinterpret_cast<float *>(ring);
-        if(warp >= 2) {
-            #pragma unroll
-            for(int j = 0; j < COLS; j++)
-                if(col0 + j < rows) partial[(col0 + j) * BM + row_in_tile] = acc[j];
-        }
-        cluster_sync();
-        if(warp >= 2) {
-            // part p of the cluster finishes rows p, p + parts, ...
-            const uint32_t base = smem_u32(partial) + row_in_tile * 4;
-            const float bias = q.bias && o < q.outputs ? ld_plain(q.bias + o) : 0.0f;
-            #pragma unroll 1
-            for(int j = part + (warp >= 6 ? parts : 0); j < rows; j += parts * (SUM / 4)) {
-                float v[MAX_CLUSTER];
-                #pragma unroll
-                for(int p = 0; p < MAX_CLUSTER; p++) v[p] = p < parts ? ld_cluster(base + j * (BM * 4), p) : 0.0f;
-                float sum = v[0];
-                #pragma unroll
-                for(int p = 1; p < MAX_CLUSTER; p++) sum += v[p];
-                if(o < q.outputs) store_out(q.y, (long long)(x_tile * BN + j) * q.y_stride + o, q.y_type, apply_act(sum + bias, q.act));
-            }
-        }
-        cluster_sync();                                      // nobody leaves while its sums are being read
-    }
-    else if(warp >= 2 && o < q.outputs) {
-        const float bias = q.bias ? ld_plain(q.bias + o) : 0.0f;
+    float *partial = reinterpret_cast<float *>(ring);        // [row of x][row of w]
+    if(warp >= 2) {
         #pragma unroll
         for(int j = 0; j < COLS; j++)
-            if(col0 + j < rows) {
-                float v = acc[j] + bias;
-                if(q.act != DLP_ACT_IDENTITY) v = apply_act(v, q.act);
-                store_out(q.y, (long long)(x_tile * BN + col0 + j) * q.y_stride + o, q.y_type, v);
-            }
+            if(col0 + j < rows) partial[(col0 + j) * BM + row_in_tile] = acc[j];
     }
+    if(parts > 1) cluster_sync();
+    else __syncthreads();
+    if(warp >= 2 && o < q.outputs) {
+        // part p of the cluster finishes rows p, p + parts, ...; of two warps with the same rows of w each takes every other one
+        const uint32_t base = smem_u32(partial) + row_in_tile * 4;
+        const float bias = q.bias ? ld_plain(q.bias + o) : 0.0f;
+        const int step = parts * (SUM / 4);
+        int j = part + (warp >= 6 ? parts : 0);
+        long long at = (long long)(x_tile * BN + j) * q.y_stride + o;
+        #pragma unroll 1
+        for(; j < rows; j += step, at += step * q.y_stride) {
+            float v;
+            if(parts > 1) {
+                float p[MAX_CLUSTER];
+                #pragma unroll
+                for(int i = 0; i < MAX_CLUSTER; i++) p[i] = i < parts ? ld_cluster(base + j * (BM * 4), i) : 0.0f;
+                v = p[0];
+                #pragma unroll
+                for(int i = 1; i < MAX_CLUSTER; i++) v += p[i];
+            }
+            else v = partial[j * BM + row_in_tile];
+            store_out(q.y, at, q.y_type, apply_act(v + bias, q.act));
+        }
+    }
+    if(parts > 1) cluster_sync();                            // nobody leaves while its sums are being read
 }
 
 // ---------------------------------------------------------------------------------------------- host
