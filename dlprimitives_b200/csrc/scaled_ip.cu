@@ -38,13 +38,12 @@ struct Params {
 
 // Warps that sum and store, beside the two that copy and issue: four have a quarter of the tile's rows each; with many columns eight, half of
 // the columns each.
-constexpr int sum_warps_for(int bn) { return bn >= 64 ? 8 : 4; }
+constexpr int sum_warps_for(int bn) { return bn == 64 ? 8 : 4; }
 constexpr int threads_for(int bn) { return 64 + 32 * sum_warps_for(bn); }
-// Blocks on an SM, and the ring's stages: what bounds this kernel is the stream of weights, and two blocks with half of the shared memory each
-// fill one another's pauses (48 rows, 4096 -> 24576: one block of eight stages 32.5 us, two of four 25.6).
-constexpr int blocks_for(int bn) { return bn <= 64 ? 2 : 1; }
+// Two blocks on an SM, with half of its shared memory each: what bounds this kernel is the stream of weights, and they fill one another's pauses.
+constexpr int PER_SM = 2;
 constexpr int fixed_for(int bn) { return 2048 + 2 * SC_CHUNK * bn * 4; }                          // alignment slack, barriers, scales
-constexpr int stages_for(int bn) { return std::min(MAX_STAGES, ((SMEM_LIMIT + 1024) / blocks_for(bn) - 1024 - fixed_for(bn)) / ((BM + bn) * BK)); }
+constexpr int stages_for(int bn) { return std::min(MAX_STAGES, ((SMEM_LIMIT + 1024) / PER_SM - 1024 - fixed_for(bn)) / ((BM + bn) * BK)); }
 
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void *tmap, int x, int y, uint32_t bar)
 {
@@ -67,11 +66,11 @@ __device__ __forceinline__ void store_out(void *y, long long at, int type, float
 
 // A tile is 128 rows of w by BN rows of x.
 template<int BN>
-__global__ void __launch_bounds__(threads_for(BN), blocks_for(BN))
+__global__ void __launch_bounds__(threads_for(BN), PER_SM)
 scaled_ip_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, const Params q, int *status)
 {
     extern __shared__ unsigned char smem_raw[];
-    constexpr int ACC = 256 * (3 - blocks_for(BN)) / BN > 4 ? 4 : 256 * (3 - blocks_for(BN)) / BN;      // accumulators in tensor memory
+    constexpr int ACC = 4;                                   // accumulators in tensor memory
     constexpr int SUM = sum_warps_for(BN), SUM_THREADS = 32 * SUM, COLS = BN * 4 / SUM;      // columns of a summing warp
     constexpr int TMEM_COLS = ACC * BN;
     constexpr int S = stages_for(BN), STAGE_BYTES = (BM + BN) * BK;
@@ -120,7 +119,7 @@ scaled_ip_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
             int kb = 0;
             #pragma unroll 1
             for(; kb < kblocks; kb++) {
-                if(!mbar_wait(empty0 + 8 * s, phase, abort_flag, status, SIP_EMPTY)) break;
+                if(!wait_quietly(empty0 + 8 * s, phase, abort_flag, status, SIP_EMPTY)) break;
                 mbar_arrive_expect_tx(&sh->full[s], STAGE_BYTES);
                 tma_load_2d(ring0 + s * STAGE_BYTES, &tm_w, (kb0 + kb) * BK, w_tile * BM, full0 + 8 * s);
                 tma_load_2d(ring0 + s * STAGE_BYTES + BM * BK, &tm_x, (kb0 + kb) * BK, x_tile * BN, full0 + 8 * s);
@@ -146,9 +145,9 @@ scaled_ip_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
             uint32_t s = 0, phase = 0, b = 0, b_phase = 1;
             #pragma unroll 1
             for(int kb = 0; kb < kblocks; kb++) {
-                if(!mbar_wait(acc_empty0 + 8 * b, b_phase, abort_flag, status, SIP_ACC_EMPTY)) break;
+                if(!wait_quietly(acc_empty0 + 8 * b, b_phase, abort_flag, status, SIP_ACC_EMPTY)) break;
                 const uint32_t wd = ring0 + s * (STAGE_BYTES >> 4), xd = wd + (BM * BK >> 4), d = tmem_base + b * BN;
-                if(!mbar_wait(full0 + 8 * s, phase, abort_flag, status, SIP_FULL)) break;
+                if(!wait_quietly(full0 + 8 * s, phase, abort_flag, status, SIP_FULL)) break;
                 tc_fence_after();
                 #pragma unroll
                 for(int j = 0; j < 4; j++)
@@ -190,11 +189,10 @@ scaled_ip_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
                 if(kb + SC_CHUNK < kblocks) fetch(kb + SC_CHUNK);
             }
             // (no vote: should the wait give up, the others do so at once, and what is read means nothing)
-            if(lane == 0) mbar_wait(acc_full0 + 8 * b, b_phase, abort_flag, status, SIP_ACC_FULL);
-            __syncwarp();
+            warp_wait_quietly(acc_full0 + 8 * b, b_phase, abort_flag, status, SIP_ACC_FULL, lane == 0);
             tc_fence_after();
             const uint32_t taddr = tmem_base + (uint32_t(quad * 32) << 16) + b * BN + col0;
-            constexpr int W = BN == 128 ? 32 : 16;
+            constexpr int W = 16;
             #pragma unroll
             for(int g = 0; g < COLS / W; g++) {
                 uint32_t v[W];
@@ -203,7 +201,7 @@ scaled_ip_few_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_cons
                 if(g + 1 == COLS / W) {
                     tc_fence_before();
                     __syncwarp();
-                    if(lane == 0) mbar_arrive(acc_empty0 + 8 * b);
+                    arrive_if(lane == 0, acc_empty0 + 8 * b);
                 }
                 #pragma unroll
                 for(int j = 0; j < W; j += 4) {
@@ -317,29 +315,55 @@ dlp_status encode_result(CUtensorMap &map, const Problem &p)
     return encode_2d(map, type, p.y, p.outputs, p.rows, p.y_stride * size, 128 / size, 32);
 }
 
-template<int BN> static dlp_status launch(const Problem &p, cudaStream_t stream)
+// Parts of K that fill the places on the SMs.
+static int few_parts(const Problem &p, int bn)
+{
+    const long long tiles = (long long)ceil_div(p.outputs, BM) * ceil_div(p.rows, bn), slots = sm_count() * 2;
+    int parts = 1;
+    while(parts < MAX_CLUSTER && parts * 2 <= p.kblocks && tiles * parts * 2 <= slots) parts *= 2;
+    return parts;
+}
+
+template<int BN> static dlp_status launch_few(const Problem &p, cudaStream_t stream)
 {
     dlp_status st = allow_shared<scaled_ip_few_kernel<BN>>(SMEM_LIMIT);
     if(st != DLP_OK) return st;
     int *status = device_status_word();
     if(!status) return fail(DLP_CUDA_ERROR, "cannot resolve the device status word");
-    const int w_tiles = ceil_div(p.outputs, BM), x_tiles = ceil_div(p.rows, BN), slots = sm_count() * blocks_for(BN);
-    // parts of K until the places on the SMs are taken
-    int parts = 1;
-    while(parts < MAX_CLUSTER && parts * 2 <= p.kblocks && (long long)w_tiles * x_tiles * parts * 2 <= slots) parts *= 2;
+    const int x_tiles = ceil_div(p.rows, BN), parts = few_parts(p, BN);
     const Params q = { p.x_scales, p.w_scales, p.bias, p.y, p.x_scale_stride, p.w_scale_stride, p.y_stride, p.rows, p.outputs, p.kblocks,
                        ceil_div(p.kblocks, parts), x_tiles, p.y_type, p.act };
     CUtensorMap mx, mw;
     st = encode_operand(mx, p.x, p.x_stride, p.rows, p.inputs, BN);
     if(st == DLP_OK) st = encode_operand(mw, p.w, p.w_stride, p.outputs, p.inputs, BM);
     if(st != DLP_OK) return st;
-    const long long blocks = (long long)w_tiles * x_tiles * parts;
+    const long long blocks = (long long)ceil_div(p.outputs, BM) * x_tiles * parts;
     DLP_REQUIRE(blocks < (1ll << 31), "too many tiles");
     // (a short part of K needs no more stages than it has blocks; the places left let the next kernel's blocks be set up early)
     const int smem = fixed_for(BN) + std::max(std::min(stages_for(BN), q.per_part), ceil_div(BN * BM * 4, (BM + BN) * BK)) * (BM + BN) * BK;
-    DLP_LAUNCH_PDL(launch_pdl_cluster(blocks <= slots, parts, scaled_ip_few_kernel<BN>, unsigned(blocks), threads_for(BN), smem, stream, mw, mx, q, status),
-                   "scaled_ip_few_kernel");
+    note_route("scaled_few", BN, parts);
+    DLP_LAUNCH_PDL(launch_pdl_cluster(blocks <= sm_count() * 2, parts, scaled_ip_few_kernel<BN>, unsigned(blocks), threads_for(BN), smem, stream, mw, mx, q,
+                                      status), "scaled_ip_few_kernel");
     return DLP_OK;
+}
+
+// Which kernel.  Up to 64 rows one tile of the few-rows kernel covers them all.  Beyond, it is measured time per block of K and round of tiles (us,
+// at full clocks): 0.64 for its 64-column tiles, two on an SM, which can be cut along K; 0.32 and 0.555 for pair tiles of 128 and 256 outputs, which
+// cannot, and have an end of 0.5 and 1.5 a round.  (Measured, 4096 inputs: 256 rows to 24576 outputs 67, 35, 42; 8192 inputs to 1000: 10.9, 26, 38;
+// 4096 rows to 24576: pair 435 and 407, and at 8192 rows 944 and 873, where the card's power limit holds both back.)
+static dlp_status dispatch(const Problem &p, cudaStream_t stream)
+{
+    if(p.rows <= 16) return launch_few<16>(p, stream);
+    if(p.rows <= 32) return launch_few<32>(p, stream);
+    if(p.rows <= 64) return launch_few<64>(p, stream);
+    const auto rounds = [](long long tiles, int places) { return double((tiles + places - 1) / places); };
+    const int parts = few_parts(p, 64);
+    const double few = rounds((long long)ceil_div(p.outputs, BM) * ceil_div(p.rows, 64) * parts, sm_count() * 2) * ceil_div(p.kblocks, parts) * 0.64;
+    const long long row_tiles = ceil_div(p.rows, 2 * BM);
+    const double narrow = rounds(row_tiles * ceil_div(p.outputs, 128), sm_count() / 2) * (p.kblocks * 0.32 + 0.5);
+    const double wide = rounds(row_tiles * ceil_div(p.outputs, 256), sm_count() / 2) * (p.kblocks * 0.555 + 1.5);
+    if(few <= narrow && few <= wide) return launch_few<64>(p, stream);
+    return launch_pair(p, narrow < wide ? 128 : 256, stream);
 }
 
 } // namespace sip
@@ -369,12 +393,7 @@ dlp_status dlp_scaled_ip_fwd(const dlp_scaled_ip_args *args, void *stream)
                 "a tensor is not aligned to its elements");
     const sip::Problem p = { x, w, x_stride, w_stride, x_scales, w_scales, bias, y, x_scale_stride, w_scale_stride, y_stride, rows, inputs, outputs,
                              kblocks, y_type, activation };
-    cudaStream_t s = (cudaStream_t)stream;
-    if(rows > 128) return sip::launch_pair(p, s);
-    if(rows <= 16) return sip::launch<16>(p, s);
-    if(rows <= 32) return sip::launch<32>(p, s);
-    if(rows <= 64) return sip::launch<64>(p, s);
-    return sip::launch<128>(p, s);
+    return sip::dispatch(p, (cudaStream_t)stream);
 }
 
 } // extern "C"

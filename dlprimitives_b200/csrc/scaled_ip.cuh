@@ -29,7 +29,47 @@ struct Problem {
 dlp_status encode_operand(CUtensorMap &map, const void *p, long long stride, int rows, int cols, int box_rows);
 // the result in boxes of 128 bytes x 32 rows, 128-byte swizzled; its rows are on 16-byte boundaries
 dlp_status encode_result(CUtensorMap &map, const Problem &p);
-dlp_status launch_pair(const Problem &p, cudaStream_t stream);
+dlp_status launch_pair(const Problem &p, int bn, cudaStream_t stream);        // bn: 128 or 256 outputs to a tile
+
+// Bounded wait, as mbar_wait, for kernels whose other warps need the issue slots: a try that may suspend the thread for 2 us costs none of them,
+// where one that comes back at once, asked again and again, took a fifth.
+__device__ __forceinline__ bool wait_quietly(uint32_t bar, uint32_t parity, int *abort_flag, int *status, int code)
+{
+    if(mbar_try_wait(bar, parity)) return true;
+    const long long t0 = global_ns();
+    #pragma unroll 1
+    for(;;) {
+        uint32_t ok;
+        asm volatile("{\n\t.reg .pred p;\n\t"
+                     "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 2000;\n\t"
+                     "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if(ok) return true;
+        if(*(volatile int *)abort_flag) return false;
+        if(global_ns() - t0 > WAIT_LIMIT_NS) {
+            *(volatile int *)abort_flag = 1;
+            atomicCAS(status, 0, code);
+            return false;
+        }
+    }
+}
+// The same by one lane for its warp (leader: lane 0), for the innermost loops.  Straight-line code as long as the barrier is complete, and nobody
+// votes: when the limit runs out the abort flag is raised, and the caller looks at it where it matters; what it reads until then means nothing.
+__device__ __forceinline__ void warp_wait_quietly(uint32_t bar, uint32_t parity, int *abort_flag, int *status, int code, bool leader)
+{
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p, l;\n\t"
+                 "setp.ne.u32 l, %3, 0;\n\t"
+                 "setp.eq.u32 p, %3, 0;\n\t"
+                 "@l mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity), "r"(uint32_t(leader)) : "memory");
+    if(!ok) wait_quietly(bar, parity, abort_flag, status, code);
+    __syncwarp();
+}
+// arrival of one lane, without a branch
+__device__ __forceinline__ void arrive_if(bool mine, uint32_t bar)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(bar), "r"(uint32_t(mine)) : "memory");
+}
 
 __device__ __forceinline__ void cluster_sync()
 {

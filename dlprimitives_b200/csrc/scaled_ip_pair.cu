@@ -59,7 +59,10 @@ __device__ __forceinline__ void commit_pair(uint32_t bar)
 }
 // Relaxed: what it says is that tensor memory has been read, which the tcgen05 fence before it orders.  A release would wait for the scale copies
 // that the thread has under way (1000 cycles a block of K).
-__device__ __forceinline__ void arrive_at(uint32_t remote) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory"); }
+__device__ __forceinline__ void arrive_at(bool mine, uint32_t remote)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t@p mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n\t}" ::"r"(remote), "r"(uint32_t(mine)) : "memory");
+}
 constexpr int FIXED_BYTES = 2048 + SUM_WARPS * STORE_BYTES + 2 * SCALE_BYTES;       // alignment slack, barriers, store boxes, scales
 constexpr int stages_for(int bn) { return std::min(MAX_STAGES, (SMEM_LIMIT - FIXED_BYTES) / ((BM + bn / 2) * BK)); }
 
@@ -127,7 +130,7 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
                     const int x_row = w.row * 2 * BM + int(rank) * BM, w_row = w.col * BN + int(rank) * (BN / 2);
                     #pragma unroll 1
                     for(int kb = 0; kb < kblocks; kb++) {
-                        if(!mbar_wait(empty0 + 8 * s, phase, abort_flag, status, SIP_EMPTY)) { live = false; break; }
+                        if(!wait_quietly(empty0 + 8 * s, phase, abort_flag, status, SIP_EMPTY)) { live = false; break; }
                         const uint32_t slot = ring0 + s * STAGE_BYTES, bar = full0 + 8 * s;
                         if(rank == 0) mbar_arrive_expect_tx(&sh->full[s], 2 * STAGE_BYTES);
                         tma_load_pair(slot, &tm_x, kb * BK, x_row, bar);
@@ -159,9 +162,9 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
                 #pragma unroll 1
                 for(long long it = 0; it < total; it++) {
                     // (the operands have been there for a while; the accumulator is what is waited for)
-                    if(!mbar_wait(full0 + 8 * s, phase, abort_flag, status, SIP_FULL)) break;
+                    if(!wait_quietly(full0 + 8 * s, phase, abort_flag, status, SIP_FULL)) break;
                     const uint32_t xd = ring + s * (STAGE_BYTES >> 4), wd = xd + (X_BYTES >> 4), d = tmem_base + b * BN;
-                    if(!mbar_wait(acc_empty0 + 8 * b, b_phase, abort_flag, status, SIP_ACC_EMPTY)) break;
+                    if(!wait_quietly(acc_empty0 + 8 * b, b_phase, abort_flag, status, SIP_ACC_EMPTY)) break;
                     tc_fence_after();
                     #pragma unroll
                     for(int j = 0; j < 4; j++)
@@ -188,7 +191,8 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
                 const float *xs = q.x_scales + row, *ws0 = q.w_scales + block0 * q.w_scale_stride, *ws1 = q.w_scales + block1 * q.w_scale_stride;
                 #pragma unroll 1
                 for(int kb0 = 0; kb0 < kblocks; kb0 += CHUNK) {
-                    if(!warp_wait(&sh->scale_empty[slot], phase, abort_flag, status, SIP_SCALE_EMPTY, lane)) { live = false; break; }
+                    warp_wait_quietly(smem_u32(&sh->scale_empty[slot]), phase, abort_flag, status, SIP_SCALE_EMPTY, lane == 0);
+                    if(*(volatile int *)abort_flag) { live = false; break; }
                     #pragma unroll
                     for(int i0 = 0; i0 < CHUNK; i0 += 4) {
                         float x0[4], x1[4], w0[4], w1[4];
@@ -224,46 +228,47 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
         const uint32_t my_store = store0 + me * STORE_BYTES;
         const uint32_t acc_empty0 = place_in(smem_u32(&sh->acc_empty[0]), 0), acc_full0 = smem_u32(&sh->acc_full[0]);
         const float2 clamp = act_clamp(q.act);
-        const uint32_t my_scales = scales0 + (half * BM + quad * 32 + lane) * 4, scale_empty0 = smem_u32(&sh->scale_empty[0]);
-        uint32_t b = 0, b_phase = 0, slot = 1, s_phase = 1, store_at = my_store;
+        const uint32_t my_scales = scales0 + (half * BM + quad * 32 + lane) * 4, scale_empty0 = smem_u32(&sh->scale_empty[0]), scale_full0 = smem_u32(&sh->scale_full[0]);
+        const bool leader = lane == 0;
+        uint32_t it = 0, slot = 1, s_phase = 1, store_at = my_store;
         bool live = true;
         for(int t = first; t < tiles && live; t += step) {
             float acc[COLS];
             #pragma unroll
             for(int j = 0; j < COLS; j++) acc[j] = 0.0f;
             #pragma unroll 1
-            for(int kb = 0; kb < kblocks; kb++) {
-                const int in = kb % CHUNK;
-                if(in == 0) {
-                    slot ^= 1;
-                    if(slot == 0) s_phase ^= 1;
-                    if(!warp_wait(&sh->scale_full[slot], s_phase, abort_flag, status, SIP_SCALE_FULL, lane)) { live = false; break; }
-                }
-                float s;
-                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(s) : "r"(my_scales + slot * SCALE_BYTES + in * (2 * BM * 4)) : "memory");
-                // (no vote: should the wait give up, what is read below means nothing, and the abort flag is seen at the next chunk)
-                if(lane == 0) mbar_wait(acc_full0 + 8 * b, b_phase, abort_flag, status, SIP_ACC_FULL);
-                __syncwarp();
-                tc_fence_after();
-                const uint32_t taddr = tmem_base + (uint32_t(quad * 32) << 16) + b * BN + half * COLS;
-                uint32_t v[2][32];
-                tmem_ld(taddr, v[0]);
-                #pragma unroll
-                for(int g = 0; g < COLS / 32; g++) {
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    if(g + 1 < COLS / 32) tmem_ld(taddr + (g + 1) * 32, v[(g + 1) & 1]);
-                    else {
-                        tc_fence_before();
-                        __syncwarp();
-                        if(lane == 0) {
-                            arrive_at(acc_empty0 + 8 * b);
-                            if(in == CHUNK - 1 || kb + 1 == kblocks) mbar_arrive(scale_empty0 + 8 * slot);
-                        }
-                    }
+            for(int left = kblocks; left > 0; left -= CHUNK) {
+                slot ^= 1;
+                if(slot == 0) s_phase ^= 1;
+                warp_wait_quietly(scale_full0 + 8 * slot, s_phase, abort_flag, status, SIP_SCALE_FULL, leader);
+                if(*(volatile int *)abort_flag) break;
+                const int n = min(left, CHUNK);
+                uint32_t scale_at = my_scales + slot * SCALE_BYTES;
+                #pragma unroll 1
+                for(int i = 0; i < n; i++, it++, scale_at += 2 * BM * 4) {
+                    const uint32_t b = it % ACC;
+                    float s;
+                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(s) : "r"(scale_at) : "memory");
+                    warp_wait_quietly(acc_full0 + 8 * b, (it / ACC) & 1, abort_flag, status, SIP_ACC_FULL, leader);
+                    tc_fence_after();
+                    const uint32_t taddr = tmem_base + (uint32_t(quad * 32) << 16) + b * BN + half * COLS;
+                    uint32_t v[2][32];
+                    tmem_ld(taddr, v[0]);
                     #pragma unroll
-                    for(int j = 0; j < 32; j++) acc[g * 32 + j] = fmaf(__uint_as_float(v[g & 1][j]), s, acc[g * 32 + j]);
+                    for(int g = 0; g < COLS / 32; g++) {
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                        if(g + 1 < COLS / 32) tmem_ld(taddr + (g + 1) * 32, v[(g + 1) & 1]);
+                        else {
+                            tc_fence_before();
+                            __syncwarp();
+                            arrive_at(leader, acc_empty0 + 8 * b);
+                        }
+                        #pragma unroll
+                        for(int j = 0; j < 32; j++) acc[g * 32 + j] = fmaf(__uint_as_float(v[g & 1][j]), s, acc[g * 32 + j]);
+                    }
                 }
-                if(++b == ACC) { b = 0; b_phase ^= 1; }
+                __syncwarp();
+                arrive_if(leader, scale_empty0 + 8 * slot);
             }
             live = live && !*(volatile int *)abort_flag;
             if(!live) break;
@@ -427,9 +432,10 @@ template<int BN> dlp_status launch_bn(const Problem &p, cudaStream_t stream)
 
 } // namespace
 
-dlp_status launch_pair(const Problem &p, cudaStream_t stream)
+dlp_status launch_pair(const Problem &p, int bn, cudaStream_t stream)
 {
-    return launch_bn<256>(p, stream);
+    note_route("scaled_pair", bn, 1);
+    return bn == 256 ? launch_bn<256>(p, stream) : launch_bn<128>(p, stream);
 }
 
 } // namespace sip

@@ -56,7 +56,7 @@ DLP_API const char *dlp_version(void);
 DLP_API uint64_t dlp_launch_count(void);
 
 /* What the calling thread's last dense contraction (GEMM, InnerProduct, convolution but depthwise and fp32 Winograd) was handed to, as
- * "kernel column-tile parts-of-K": general_{gather,strided,taps,rowtaps}, stream_{k,units,copy}, staged, pointwise, ffma.  For tests and
+ * "kernel column-tile parts-of-K": general_{gather,strided,taps,rowtaps}, stream_{k,units,copy}, staged, pointwise, ffma, scaled_{few,pair}.  For tests and
  * timing; valid until the thread's next call of it. */
 DLP_API const char *dlp_last_route(void);
 
