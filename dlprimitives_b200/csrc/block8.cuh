@@ -20,76 +20,181 @@ template<> __device__ __forceinline__ float from_float<float>(float v) { return 
 template<> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 template<> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// Eight consecutive elements; VEC: 16-byte accesses, all eight there (p aligned to 16 bytes).  Otherwise one by one, the first `count` of them, and
-// zeros for the rest.
-template<typename T, bool VEC> __device__ __forceinline__ void load8(const T *p, int count, float (&v)[8])
+// ---- Rows, eight consecutive elements to a lane: lane l of WIDTH (32, or 16: two rows to a warp) has the elements from column c = c0 + 8 l.
+// Memory is read and written in 16-byte pieces on their boundaries, also where a row starts off one (any length and stride of 16-bit elements):
+// then a lane's elements lie in its own pieces and the first one of the lane after it, m elements on.  Pieces that reach beyond the row, into
+// memory that is not this call's, go element by element.  All lanes take part (with c >= cols where there is nothing).
+template<typename T> constexpr int PIECE = 16 / int(sizeof(T));               // elements of a piece
+template<typename T> constexpr int WORDS = 2 * int(sizeof(T));                // 32-bit words of eight elements
+template<typename T> __device__ __forceinline__ int off_boundary(const T *row) { return int(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T)); }
+
+// N words from `bytes` (even, under 16) on in N + 4
+template<int N> __device__ __forceinline__ void shift_words(uint32_t (&w)[N + 4], int bytes)
 {
-    if(VEC) {
-        union { uint4 w[sizeof(T) / 2]; T e[8]; } u;
+    #pragma unroll
+    for(int i = 0; i < N + 2; i++) w[i] = bytes & 8 ? w[i + 2] : w[i];
+    #pragma unroll
+    for(int i = 0; i < N + 1; i++) w[i] = bytes & 4 ? w[i + 1] : w[i];
+    #pragma unroll
+    for(int i = 0; i < N; i++) w[i] = bytes & 2 ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+}
+// A load in three steps, so that a thread can ask for all it reads before it waits for any of it: ask() for the whole pieces (predicated loads, no
+// branch), patch() for the elements of pieces that the row's ends cut, settle() when the values are used.
+template<typename T, bool OFF, int WIDTH = 32> struct Row8 {
+    uint32_t w[WORDS<T> + (OFF ? 4 : 0)];
+    static __device__ __forceinline__ int lane() { return threadIdx.x & (WIDTH - 1); }
+    __device__ __forceinline__ void piece(int i, const T *row, int e, int cols, bool wanted)
+    {
+        w[i] = w[i + 1] = w[i + 2] = w[i + 3] = 0;
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\t@p ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+                     : "+r"(w[i]), "+r"(w[i + 1]), "+r"(w[i + 2]), "+r"(w[i + 3])
+                     : "l"(row + e), "r"(uint32_t(wanted && e >= 0 && e + PIECE<T> <= cols)) : "memory");
+    }
+    __device__ __forceinline__ void ask(const T *row, int c, int cols)
+    {
+        const int m = OFF ? off_boundary(row) : 0;
         #pragma unroll
-        for(int i = 0; i < int(sizeof(T)) / 2; i++) u.w[i] = ld_plain(reinterpret_cast<const uint4 *>(p) + i);
+        for(int i = 0; i < WORDS<T>; i += 4) piece(i, row, c - m + i / 4 * PIECE<T>, cols, true);
+        if(OFF) piece(WORDS<T>, row, c - m + 8, cols, m != 0 && lane() == WIDTH - 1);
+    }
+    __device__ __forceinline__ void patch(const T *row, int c, int cols)
+    {
+        const int m = OFF ? off_boundary(row) : 0, first = c - lane() * 8;
+        if(first - m >= 0 && first + WIDTH * 8 + (OFF ? PIECE<T> : 0) <= cols) return;       // the whole warp is inside
+        #pragma unroll
+        for(int i = 0; i < WORDS<T> + (OFF ? 4 : 0); i += 4) {
+            const int e = c - m + i / 4 * PIECE<T>;
+            if((e >= 0 && e + PIECE<T> <= cols) || e + PIECE<T> <= 0 || e >= cols || (i == WORDS<T> && (m == 0 || lane() != WIDTH - 1))) continue;
+            union { T e[PIECE<T>]; uint32_t w[4]; } u;
+            #pragma unroll
+            for(int k = 0; k < 4; k++) u.w[k] = 0;
+            #pragma unroll
+            for(int k = 0; k < PIECE<T>; k++)
+                if(e + k >= 0 && e + k < cols) u.e[k] = ld_plain(row + e + k);
+            #pragma unroll
+            for(int k = 0; k < 4; k++) w[i + k] = u.w[k];
+        }
+    }
+    // the eight elements; all lanes take part
+    __device__ __forceinline__ void settle(const T *row, float (&v)[8])
+    {
+        if constexpr(OFF) {
+            const int m = off_boundary(row);
+            #pragma unroll
+            for(int i = 0; i < 4; i++) {
+                const uint32_t next = __shfl_down_sync(0xffffffffu, w[i], 1, WIDTH);
+                w[WORDS<T> + i] = lane() == WIDTH - 1 ? w[WORDS<T> + i] : next;
+            }
+            shift_words<WORDS<T>>(w, m * int(sizeof(T)));
+        }
+        union { uint32_t w[WORDS<T>]; T e[8]; } u;
+        #pragma unroll
+        for(int i = 0; i < WORDS<T>; i++) u.w[i] = w[i];
         #pragma unroll
         for(int j = 0; j < 8; j++) v[j] = to_float(u.e[j]);
     }
+};
+
+template<typename T> __device__ __forceinline__ void store_piece(T *row, int e, int from, int cols, const uint32_t *w)
+{
+    if(e >= from && e + PIECE<T> <= cols) *reinterpret_cast<uint4 *>(row + e) = make_uint4(w[0], w[1], w[2], w[3]);
     else {
+        union { uint32_t w[4]; T e[PIECE<T>]; } u;
         #pragma unroll
-        for(int j = 0; j < 8; j++) v[j] = j < count ? to_float(ld_plain(p + j)) : 0.0f;
+        for(int i = 0; i < 4; i++) u.w[i] = w[i];
+        #pragma unroll
+        for(int i = 0; i < PIECE<T>; i++)
+            if(e + i >= from && e + i < cols) row[e + i] = u.e[i];
     }
 }
-template<typename T, bool VEC> __device__ __forceinline__ void store8(T *p, int count, const float (&v)[8])
+template<typename T> __device__ __forceinline__ void store_words(T *row, int c, int cols, const uint32_t (&w)[WORDS<T>])
 {
-    if(VEC) {
-        union { uint4 w[sizeof(T) / 2]; T e[8]; } u;
+    if(c < cols) {
         #pragma unroll
-        for(int j = 0; j < 8; j++) u.e[j] = from_float<T>(v[j]);
-        #pragma unroll
-        for(int i = 0; i < int(sizeof(T)) / 2; i++) reinterpret_cast<uint4 *>(p)[i] = u.w[i];
+        for(int g = 0; g < WORDS<T> / 4; g++) store_piece(row, c + g * PIECE<T>, 0, cols, w + g * 4);
     }
-    else {
+}
+template<typename T> __device__ __forceinline__ void store_words_off(T *row, int c, int cols, const uint32_t (&w)[WORDS<T>])
+{
+    // a lane stores the pieces that begin with the last m elements of the lane before; the first and the last lane what is theirs of the outer ones
+    const int m = off_boundary(row), lane = threadIdx.x & 31;
+    uint32_t all[WORDS<T> + 4];
+    #pragma unroll
+    for(int i = 0; i < WORDS<T>; i++) all[i + 4] = w[i];
+    #pragma unroll
+    for(int i = 0; i < 4; i++) all[i] = __shfl_up_sync(0xffffffffu, w[WORDS<T> - 4 + i], 1);
+    shift_words<WORDS<T>>(all, 16 - m * int(sizeof(T)));
+    #pragma unroll
+    for(int g = 0; g < WORDS<T> / 4; g++) store_piece(row, c - m + g * PIECE<T>, lane == 0 ? c : 0, cols, all + g * 4);
+    if(lane == 31) {
+        union { uint32_t w[4]; T e[PIECE<T>]; } u;
         #pragma unroll
-        for(int j = 0; j < 8; j++)
-            if(j < count) p[j] = from_float<T>(v[j]);
+        for(int i = 0; i < 4; i++) u.w[i] = w[WORDS<T> - 4 + i];
+        #pragma unroll
+        for(int i = 0; i < PIECE<T>; i++)
+            if(i >= PIECE<T> - m && c + 8 - PIECE<T> + i < cols) row[c + 8 - PIECE<T> + i] = u.e[i];
     }
+}
+// OFF: the row may start off a 16-byte boundary
+template<typename T, bool OFF> __device__ __forceinline__ void store8(T *row, int c, int cols, const float (&v)[8])
+{
+    union { uint32_t w[WORDS<T>]; T e[8]; } u;
+    #pragma unroll
+    for(int j = 0; j < 8; j++) u.e[j] = from_float<T>(v[j]);
+    if(OFF && off_boundary(row) != 0) store_words_off(row, c, cols, u.w);
+    else store_words(row, c, cols, u.w);
 }
 
 // The 8-bit form of a block of values v is a scale s = max|v| / 448 (448: the largest e4m3) and the numbers e4m3(v / s): the largest value
 // meets the largest number.  s is no smaller than 2^-126, so that a block of zeros, or of subnormals, has a finite 1 / s; a NaN or
 // an infinity in the block makes s NaN or infinite and with it whatever is computed from the block.
-// Largest magnitude of the thread's values, as bits: magnitudes are ordered as their bits are, a NaN above all of them.
+// Largest magnitude of the thread's values, as bits (magnitudes are ordered as their bits are); a NaN if one of them is.
 __device__ __forceinline__ unsigned magnitude_bits(const float (&v)[8])
 {
-    unsigned m = 0;
+    float m = fabsf(v[0]);
     #pragma unroll
-    for(int j = 0; j < 8; j++) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
-    return m;
+    for(int j = 1; j < 8; j++) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v[j])));
+    return __float_as_uint(m);
 }
+// The quotient by 448 is the product with its reciprocal, corrected by the remainder: rounded as a division would, without its length.
 __device__ __forceinline__ float block_scale(unsigned magnitude)
 {
-    const float s = __uint_as_float(magnitude) / 448.0f;
-    return s < 1.17549435e-38f ? 1.17549435e-38f : s;
+    const float m = __uint_as_float(magnitude);
+    const float s0 = m * (1.0f / 448.0f), s = fmaf(fmaf(-448.0f, s0, m), 1.0f / 448.0f, s0);
+    return m < 5.2656e-36f ? 1.17549435e-38f : (magnitude < 0x7f800000u ? s : m);          // 448 * 2^-126 (under it 2^-126); infinite and NaN stay
 }
-// Eight numbers of the block, the first in the lowest byte.  v * (1 / s) is within one and a half units in the last place of v / s in fp32, a
-// twenty-thousandth part of a step of e4m3: only a value that close to the middle of two numbers may go to the other one.
-__device__ __forceinline__ uint2 pack_e4m3(const float (&v)[8], float inverse_scale)
+// Eight numbers of the block, the first in the lowest byte: v / s, by a product with the approximate 1 / s and a correction of its remainder (a Newton step
+// of the quotient, after which it is the rounded one but for rare last units), then to the nearest e4m3, ties to even.
+__device__ __forceinline__ uint2 pack_e4m3(const float (&v)[8], float scale)
 {
+    // (an infinite scale takes the correction out: finite values give 0, infinite ones and NaN a NaN)
+    const float back = scale < __int_as_float(0x7f800000) ? -scale : 0.0f;
+    float inverse;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(inverse) : "f"(scale));
     uint32_t w[2];
     #pragma unroll
     for(int i = 0; i < 2; i++) {
+        float q[4];
+        #pragma unroll
+        for(int j = 0; j < 4; j++) {
+            const float q0 = v[4 * i + j] * inverse;
+            q[j] = fmaf(fmaf(back, q0, v[4 * i + j]), inverse, q0);
+        }
         unsigned short a, b;
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(a) : "f"(v[4 * i + 1] * inverse_scale), "f"(v[4 * i] * inverse_scale));
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b) : "f"(v[4 * i + 3] * inverse_scale), "f"(v[4 * i + 2] * inverse_scale));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(a) : "f"(q[1]), "f"(q[0]));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b) : "f"(q[3]), "f"(q[2]));
         w[i] = uint32_t(a) | uint32_t(b) << 16;
     }
     return make_uint2(w[0], w[1]);
 }
-// VEC: one 8-byte store (p aligned to 8 bytes)
-template<bool VEC> __device__ __forceinline__ void store_e4m3(unsigned char *p, int count, uint2 w)
+// aligned: the row is on an 8-byte boundary
+__device__ __forceinline__ void store_e4m3(unsigned char *row, int c, int cols, bool aligned, uint2 w)
 {
-    if(VEC) *reinterpret_cast<uint2 *>(p) = w;
+    if(aligned && c + 8 <= cols) *reinterpret_cast<uint2 *>(row + c) = w;
     else {
         #pragma unroll
         for(int j = 0; j < 8; j++)
-            if(j < count) p[j] = (unsigned char)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
+            if(c + j < cols) row[c + j] = (unsigned char)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));
     }
 }
 

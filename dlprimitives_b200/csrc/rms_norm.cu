@@ -1,6 +1,8 @@
 // Root-mean-square norm of rows, with the addition of a residual before it and an 8-bit form of the result:
 //     h = x + residual,   y = h / sqrt(mean(h^2) + eps) * weight.
-// The row's sum of squares has to be complete before the first output, so a row is read twice: simple, the second time from L2.
+// A block of threads has a row in its registers between the sum of squares and the outputs, so that a row is read once (up to 32768 columns; longer
+// ones are read a second time, from L2).  What bounds it is memory: 8192 x 5120 bf16 with residual, 8-bit output: NORM_A.
+// Rows that start off 16-byte boundaries are read and written in aligned pieces all the same (block8.cuh): NORM_B.
 #include "block8.cuh"
 
 namespace dlp {
@@ -17,77 +19,188 @@ struct NormArgs {
 
 constexpr int MAX_THREADS = 512;
 
-// A block of threads per row; a thread takes eight consecutive columns at a time, so that sixteen lanes hold a block of the 8-bit form.
-template<typename T, bool VEC>
-__global__ void __launch_bounds__(MAX_THREADS) rms_norm_kernel(const NormArgs a)
+// Sum over the block; `part` is used in turn from call to call, so that one barrier a call is enough.
+__device__ __forceinline__ float block_sum(float v, float (&part)[MAX_THREADS / 32])
+{
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    #pragma unroll
+    for(int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if(warps == 1) return v;
+    if(lane == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = (lane & (MAX_THREADS / 32 - 1)) < warps ? part[lane & (MAX_THREADS / 32 - 1)] : 0.0f;
+    #pragma unroll
+    for(int o = MAX_THREADS / 64; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// 1 / sqrt(v), with a Newton step for the last bits of the approximation
+__device__ __forceinline__ float inverse_root(float v)
+{
+    const float f = rsqrtf(v);
+    return v < __int_as_float(0x7f800000) ? fmaf(0.5f * f, fmaf(-v * f, f, 1.0f), f) : f;
+}
+
+// What becomes of eight values h of a row: total, and the output in its type.
+template<typename T, bool OFF>
+__device__ __forceinline__ void norm_out(const NormArgs &a, long long row, int c, float (&v)[8], const float (&g)[8], float f)
+{
+    const int lane = threadIdx.x & 31;
+    if(a.total) store8<T, OFF>(static_cast<T *>(a.total) + row * a.total_stride, c, a.cols, v);
+    #pragma unroll
+    for(int j = 0; j < 8; j++) v[j] = v[j] * f * g[j];
+    if(a.y_type == DLP_TYPE_E4M3) {
+        const float s = block_scale(__reduce_max_sync(lane < 16 ? 0xffffu : 0xffff0000u, magnitude_bits(v)));
+        unsigned char *y = static_cast<unsigned char *>(a.y) + row * a.y_stride;
+        if((lane & 15) == 0 && c < a.cols) a.scales[(c / SCALE_BLOCK) * a.scale_stride + row] = s;
+        store_e4m3(y, c, a.cols, reinterpret_cast<uintptr_t>(y) % 8 == 0, pack_e4m3(v, s));
+    }
+    else if(a.y_type == DLP_TYPE_F32) store8<float, OFF>(static_cast<float *>(a.y) + row * a.y_stride, c, a.cols, v);
+    else if(a.y_type == DLP_TYPE_F16) store8<__half, OFF>(static_cast<__half *>(a.y) + row * a.y_stride, c, a.cols, v);
+    else store8<__nv_bfloat16, OFF>(static_cast<__nv_bfloat16 *>(a.y) + row * a.y_stride, c, a.cols, v);
+}
+
+constexpr bool half_registers(int nv, bool off) { return nv <= 2 && !off; }
+
+// NV: pieces of eight columns that a thread keeps, a block's width apart, so that a warp has 256 consecutive columns, two blocks of the 8-bit form.
+// OFF: rows of some tensor start off 16-byte boundaries.  A block takes rows in turn and asks for the next one as soon as the registers of this one's
+// words are free: the reduction, the arithmetic and the stores of a row run under the loads of the next.  The weights stay.
+template<typename T, int NV, bool OFF>
+__global__ void __launch_bounds__(MAX_THREADS, half_registers(NV, OFF) ? 2 : 1) rms_norm_kernel(const NormArgs a, int rows)
+{
+    pdl_wait();
+    __shared__ float part[2][MAX_THREADS / 32];
+    typedef Row8<T, OFF> Row;
+    const int cols = a.cols, stride = blockDim.x * 8, c0 = threadIdx.x * 8;
+    const T *weight = static_cast<const T *>(a.weight);
+    const auto x_at = [&](long long row) { return static_cast<const T *>(a.x) + row * a.x_stride; };
+    const auto r_at = [&](long long row) { return static_cast<const T *>(a.residual) + row * a.residual_stride; };
+    constexpr bool KEEP_WEIGHT = NV * WORDS<T> <= 16;        // (as far as registers go)
+    Row xw[NV], rw[NV], ww[KEEP_WEIGHT ? NV : 1];
+    auto ask = [&](long long row) {
+        #pragma unroll
+        for(int i = 0; i < NV; i++) {
+            xw[i].ask(x_at(row), c0 + i * stride, cols);
+            if(a.residual) rw[i].ask(r_at(row), c0 + i * stride, cols);
+        }
+    };
+    ask(blockIdx.x);
+    if(KEEP_WEIGHT) {
+        #pragma unroll
+        for(int i = 0; i < NV; i++) ww[KEEP_WEIGHT ? i : 0].ask(weight, c0 + i * stride, cols);
+        #pragma unroll
+        for(int i = 0; i < NV; i++) ww[KEEP_WEIGHT ? i : 0].patch(weight, c0 + i * stride, cols);
+    }
+    int turn = 0;
+    #pragma unroll 1
+    for(int row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
+        float h[NV][8], sum = 0.0f;
+        #pragma unroll
+        for(int i = 0; i < NV; i++) {
+            xw[i].patch(x_at(row), c0 + i * stride, cols);
+            if(a.residual) rw[i].patch(r_at(row), c0 + i * stride, cols);
+        }
+        #pragma unroll
+        for(int i = 0; i < NV; i++) {
+            xw[i].settle(x_at(row), h[i]);
+            if(a.residual) {
+                float b[8];
+                rw[i].settle(r_at(row), b);
+                #pragma unroll
+                for(int j = 0; j < 8; j++) h[i][j] += b[j];
+            }
+            #pragma unroll
+            for(int j = 0; j < 8; j++) sum += h[i][j] * h[i][j];
+        }
+        if(row + int(gridDim.x) < rows) ask(row + int(gridDim.x));
+        const float f = inverse_root(block_sum(sum, part[turn]) / float(cols) + a.eps);
+        #pragma unroll
+        for(int i = 0; i < NV; i++) {
+            const int c = c0 + i * stride;
+            Row w;
+            if(KEEP_WEIGHT) w = ww[KEEP_WEIGHT ? i : 0];
+            else {
+                w.ask(weight, c, cols);
+                w.patch(weight, c, cols);
+            }
+            float g[8];
+            w.settle(weight, g);
+            norm_out<T, OFF>(a, row, c, h[i], g, f);
+        }
+    }
+}
+
+// Rows of more than a block's registers: read twice, the second time from L2.
+template<typename T, bool OFF>
+__global__ void __launch_bounds__(MAX_THREADS, 2) rms_norm_long_kernel(const NormArgs a)
 {
     pdl_wait();
     __shared__ float part[MAX_THREADS / 32];
     const long long row = blockIdx.x;
-    const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
+    const int cols = a.cols, stride = blockDim.x * 8;
+    const T *x = static_cast<const T *>(a.x) + row * a.x_stride, *weight = static_cast<const T *>(a.weight);
     const T *r = a.residual ? static_cast<const T *>(a.residual) + row * a.residual_stride : nullptr;
-    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     auto fetch = [&](int c, float (&h)[8]) {
-        load8<T, VEC>(x + c, a.cols - c, h);
+        Row8<T, OFF> xw, rw;
+        xw.ask(x, c, cols);
+        if(r) rw.ask(r, c, cols);
+        xw.patch(x, c, cols);
+        xw.settle(x, h);
         if(r) {
             float b[8];
-            load8<T, VEC>(r + c, a.cols - c, b);
+            rw.patch(r, c, cols);
+            rw.settle(r, b);
             #pragma unroll
             for(int j = 0; j < 8; j++) h[j] += b[j];
         }
     };
     float sum = 0.0f;
-    for(int c = threadIdx.x * 8; c < a.cols; c += blockDim.x * 8) {
+    for(int c0 = 0; c0 < cols; c0 += stride) {
         float h[8];
-        fetch(c, h);
+        fetch(c0 + threadIdx.x * 8, h);
         #pragma unroll
         for(int j = 0; j < 8; j++) sum += h[j] * h[j];
     }
-    #pragma unroll
-    for(int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if(lane == 0) part[threadIdx.x >> 5] = sum;
-    __syncthreads();
-    sum = 0.0f;
-    for(int i = 0; i < warps; i++) sum += part[i];
-    const float f = rsqrtf(sum / float(a.cols) + a.eps);
-    // (whole blocks of lanes stay in the loop for the maximum over a block)
-    for(int c0 = 0; c0 < a.cols; c0 += blockDim.x * 8) {
+    const float f = inverse_root(block_sum(sum, part) / float(cols) + a.eps);
+    for(int c0 = 0; c0 < cols; c0 += stride) {
         const int c = c0 + threadIdx.x * 8;
-        const bool in = c < a.cols;
-        const int count = a.cols - c;
-        float v[8] = {};
-        if(in) {
-            float w[8];
-            fetch(c, v);
-            load8<T, VEC>(static_cast<const T *>(a.weight) + c, count, w);
-            if(a.total) store8<T, VEC>(static_cast<T *>(a.total) + row * a.total_stride + c, count, v);
-            #pragma unroll
-            for(int j = 0; j < 8; j++) v[j] = v[j] * f * w[j];
-        }
-        if(a.y_type == DLP_TYPE_E4M3) {
-            const unsigned m = __reduce_max_sync(lane < 16 ? 0xffffu : 0xffff0000u, magnitude_bits(v));
-            const float s = block_scale(m);
-            if(in) {
-                if((threadIdx.x & 15) == 0) a.scales[(c / SCALE_BLOCK) * a.scale_stride + row] = s;
-                store_e4m3<VEC>(static_cast<unsigned char *>(a.y) + row * a.y_stride + c, count, pack_e4m3(v, 1.0f / s));
-            }
-        }
-        else if(in) {
-            if(a.y_type == DLP_TYPE_F32) store8<float, VEC>(static_cast<float *>(a.y) + row * a.y_stride + c, count, v);
-            else if(a.y_type == DLP_TYPE_F16) store8<__half, VEC>(static_cast<__half *>(a.y) + row * a.y_stride + c, count, v);
-            else store8<__nv_bfloat16, VEC>(static_cast<__nv_bfloat16 *>(a.y) + row * a.y_stride + c, count, v);
-        }
+        float h[8], g[8];
+        Row8<T, OFF> w;
+        w.ask(weight, c, cols);
+        fetch(c, h);
+        w.patch(weight, c, cols);
+        w.settle(weight, g);
+        norm_out<T, OFF>(a, row, c, h, g, f);
     }
 }
 
-template<typename T>
-dlp_status launch_norm(const NormArgs &a, int rows, bool vec, cudaStream_t stream)
+template<typename T, int NV>
+dlp_status launch_nv(const NormArgs &a, int rows, int threads, bool off, cudaStream_t stream)
 {
-    const int threads = std::min(MAX_THREADS, round_up(ceil_div(a.cols, 8), 32));
-    const bool early = one_wave(rows, threads);
-    if(vec) DLP_LAUNCH_PDL(launch_pdl(early, rms_norm_kernel<T, true>, rows, threads, 0, stream, a), "rms_norm_kernel");
-    else DLP_LAUNCH_PDL(launch_pdl(early, rms_norm_kernel<T, false>, rows, threads, 0, stream, a), "rms_norm_kernel");
+    const int blocks = std::min(rows, sm_count() * std::max(1, (half_registers(NV, off) ? 1024 : 512) / threads));       // all of them resident
+    if(off) DLP_LAUNCH_PDL(launch_pdl(true, rms_norm_kernel<T, NV, true>, blocks, threads, 0, stream, a, rows), "rms_norm_kernel");
+    else DLP_LAUNCH_PDL(launch_pdl(true, rms_norm_kernel<T, NV, false>, blocks, threads, 0, stream, a, rows), "rms_norm_kernel");
     return DLP_OK;
+}
+template<typename T>
+dlp_status launch_norm(const NormArgs &a, int rows, bool off, cudaStream_t stream)
+{
+    // With few rows each has as many threads as it can use (latency); with many, threads that keep two pieces or more have more loads under way.
+    const int pieces = ceil_div(a.cols, 8), least = rows <= 2 * sm_count() ? 1 : 2;
+    int nv = 1;
+    while(nv < 8 && (nv < least || ceil_div(pieces, nv) > MAX_THREADS)) nv *= 2;
+    const int threads = round_up(ceil_div(pieces, nv), 32);
+    if(threads > MAX_THREADS) {
+        const bool early = one_wave(rows, MAX_THREADS);
+        if(off) DLP_LAUNCH_PDL(launch_pdl(early, rms_norm_long_kernel<T, true>, rows, MAX_THREADS, 0, stream, a), "rms_norm_long_kernel");
+        else DLP_LAUNCH_PDL(launch_pdl(early, rms_norm_long_kernel<T, false>, rows, MAX_THREADS, 0, stream, a), "rms_norm_long_kernel");
+        return DLP_OK;
+    }
+    switch(nv) {
+    case 1: return launch_nv<T, 1>(a, rows, threads, off, stream);
+    case 2: return launch_nv<T, 2>(a, rows, threads, off, stream);
+    case 4: return launch_nv<T, 4>(a, rows, threads, off, stream);
+    default: return launch_nv<T, 8>(a, rows, threads, off, stream);
+    }
 }
 
 } // namespace
@@ -101,7 +214,7 @@ dlp_status dlp_rms_norm_fwd(const dlp_rms_norm_args *args, void *stream)
 {
     DLP_REQUIRE(args != nullptr, "null arguments");
     const auto [x, residual, weight, total, y, scales, x_stride, residual_stride, total_stride, y_stride, scale_stride, rows, cols, type, y_type, eps] = *args;
-    DLP_REQUIRE(rows >= 0 && cols > 0, "bad norm shape");
+    DLP_REQUIRE(rows >= 0 && cols > 0 && cols < (1 << 30), "bad norm shape");
     DLP_REQUIRE(is_real_type(type), "the input's type must be fp32, fp16 or bf16");
     DLP_REQUIRE(is_real_type(y_type) || y_type == DLP_TYPE_E4M3, "unknown output type");
     DLP_REQUIRE(eps > 0.0f && eps < 1e30f, "eps must be positive and finite");
@@ -116,13 +229,12 @@ dlp_status dlp_rms_norm_fwd(const dlp_rms_norm_args *args, void *stream)
     DLP_REQUIRE(aligned_to(x, size) && aligned_to(weight, size) && aligned_to(y, y_size) && (!residual || aligned_to(residual, size)) &&
                 (!total || aligned_to(total, size)) && (!scales || aligned_to(scales, 4)), "a tensor is not aligned to its elements");
     NormArgs a = { x, residual, weight, total, y, scales, x_stride, residual_stride, total_stride, y_stride, scale_stride, cols, y_type, eps };
-    // 16-byte accesses (8 for the 8-bit output): every row and its end on such a boundary
-    const auto rows_on = [rows = args->rows](const void *p, long long stride, size_t element, size_t n) { return aligned_to(p, n) && (rows == 1 || stride * element % n == 0); };
-    const bool vec = cols % 8 == 0 && rows_on(x, x_stride, size, 16) && aligned_to(weight, 16) && (!residual || rows_on(residual, residual_stride, size, 16)) &&
-                     (!total || rows_on(total, total_stride, size, 16)) && rows_on(y, y_stride, y_size, y_type == DLP_TYPE_E4M3 ? 8 : 16);
-    if(type == DLP_TYPE_F32) return launch_norm<float>(a, rows, vec, (cudaStream_t)stream);
-    if(type == DLP_TYPE_F16) return launch_norm<__half>(a, rows, vec, (cudaStream_t)stream);
-    return launch_norm<__nv_bfloat16>(a, rows, vec, (cudaStream_t)stream);
+    const auto rows_on = [rows = args->rows](const void *p, long long stride, size_t element) { return aligned_to(p, 16) && (rows == 1 || stride * element % 16 == 0); };
+    const bool off = !(rows_on(x, x_stride, size) && aligned_to(weight, 16) && (!residual || rows_on(residual, residual_stride, size)) &&
+                       (!total || rows_on(total, total_stride, size)) && (y_type == DLP_TYPE_E4M3 || rows_on(y, y_stride, y_size)));
+    if(type == DLP_TYPE_F32) return launch_norm<float>(a, rows, off, (cudaStream_t)stream);
+    if(type == DLP_TYPE_F16) return launch_norm<__half>(a, rows, off, (cudaStream_t)stream);
+    return launch_norm<__nv_bfloat16>(a, rows, off, (cudaStream_t)stream);
 }
 
 } // extern "C"
