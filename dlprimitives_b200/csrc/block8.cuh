@@ -3,6 +3,7 @@
 #include "common.cuh"
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <algorithm>
 
 namespace dlp {
 
@@ -20,10 +21,39 @@ template<> __device__ __forceinline__ float from_float<float>(float v) { return 
 template<> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 template<> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// Two fp32 operations to an instruction: what bounds these kernels beside memory is the issue of instructions.
+struct Pair { unsigned long long v; };
+__device__ __forceinline__ Pair pair(float a, float b)
+{
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ Pair both(float a) { return pair(a, a); }
+__device__ __forceinline__ void apart(Pair r, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r.v)); }
+__device__ __forceinline__ Pair operator*(Pair a, Pair b)
+{
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Pair operator+(Pair a, Pair b)
+{
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c)
+{
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+
 // ---- Rows, eight consecutive elements to a lane: lane l of WIDTH (32, or 16: two rows to a warp) has the elements from column c = c0 + 8 l.
 // Memory is read and written in 16-byte pieces on their boundaries, also where a row starts off one (any length and stride of 16-bit elements):
-// then a lane's elements lie in its own pieces and the first one of the lane after it, m elements on.  Pieces that reach beyond the row, into
-// memory that is not this call's, go element by element.  All lanes take part (with c >= cols where there is nothing).
+// then a lane's elements lie in its own pieces and the first one of the lane after it, m elements on.  Stores that a row's ends cut go element by element,
+// and so do loads of pieces that reach beyond the tensor.  All lanes take part (with c >= cols where there is nothing).
 template<typename T> constexpr int PIECE = 16 / int(sizeof(T));               // elements of a piece
 template<typename T> constexpr int WORDS = 2 * int(sizeof(T));                // 32-bit words of eight elements
 template<typename T> __device__ __forceinline__ int off_boundary(const T *row) { return int(reinterpret_cast<uintptr_t>(row) % 16 / sizeof(T)); }
@@ -38,47 +68,61 @@ template<int N> __device__ __forceinline__ void shift_words(uint32_t (&w)[N + 4]
     #pragma unroll
     for(int i = 0; i < N; i++) w[i] = bytes & 2 ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
 }
-// A load in three steps, so that a thread can ask for all it reads before it waits for any of it: ask() for the whole pieces (predicated loads, no
-// branch), patch() for the elements of pieces that the row's ends cut, settle() when the values are used.
-template<typename T, bool OFF, int WIDTH = 32> struct Row8 {
-    uint32_t w[WORDS<T> + (OFF ? 4 : 0)];
+// What a row is known to be: WHOLE, on a 16-byte boundary and a multiple of eight elements long, so that a lane's eight are all there or none; or ANY.
+enum { ROW_WHOLE, ROW_ANY };
+// A load in two steps, so that a thread can ask for all it reads before it waits for any of it: ask(), and settle() when the values are used.
+template<typename T, int KIND, int WIDTH = 32> struct Row8 {
+    uint32_t w[WORDS<T> + (KIND == ROW_ANY ? 4 : 0)];
     static __device__ __forceinline__ int lane() { return threadIdx.x & (WIDTH - 1); }
-    __device__ __forceinline__ void piece(int i, const T *row, int e, int cols, bool wanted)
+    __device__ __forceinline__ void put(int i, uint4 v) { w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w; }
+    // the elements of a piece that the row's ends cut
+    __device__ __forceinline__ void cut_piece(int i, const T *row, int e, int cols)
     {
-        w[i] = w[i + 1] = w[i + 2] = w[i + 3] = 0;
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\t@p ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
-                     : "+r"(w[i]), "+r"(w[i + 1]), "+r"(w[i + 2]), "+r"(w[i + 3])
-                     : "l"(row + e), "r"(uint32_t(wanted && e >= 0 && e + PIECE<T> <= cols)) : "memory");
-    }
-    __device__ __forceinline__ void ask(const T *row, int c, int cols)
-    {
-        const int m = OFF ? off_boundary(row) : 0;
-        #pragma unroll
-        for(int i = 0; i < WORDS<T>; i += 4) piece(i, row, c - m + i / 4 * PIECE<T>, cols, true);
-        if(OFF) piece(WORDS<T>, row, c - m + 8, cols, m != 0 && lane() == WIDTH - 1);
-    }
-    __device__ __forceinline__ void patch(const T *row, int c, int cols)
-    {
-        const int m = OFF ? off_boundary(row) : 0, first = c - lane() * 8;
-        if(first - m >= 0 && first + WIDTH * 8 + (OFF ? PIECE<T> : 0) <= cols) return;       // the whole warp is inside
-        #pragma unroll
-        for(int i = 0; i < WORDS<T> + (OFF ? 4 : 0); i += 4) {
-            const int e = c - m + i / 4 * PIECE<T>;
-            if((e >= 0 && e + PIECE<T> <= cols) || e + PIECE<T> <= 0 || e >= cols || (i == WORDS<T> && (m == 0 || lane() != WIDTH - 1))) continue;
-            union { T e[PIECE<T>]; uint32_t w[4]; } u;
-            #pragma unroll
-            for(int k = 0; k < 4; k++) u.w[k] = 0;
+        union { T e[PIECE<T>]; uint4 w; } u;
+        u.w = make_uint4(0, 0, 0, 0);
+        if(e >= 0 && e + PIECE<T> <= cols) u.w = ld_plain(reinterpret_cast<const uint4 *>(row + e));
+        else {
             #pragma unroll
             for(int k = 0; k < PIECE<T>; k++)
                 if(e + k >= 0 && e + k < cols) u.e[k] = ld_plain(row + e + k);
-            #pragma unroll
-            for(int k = 0; k < 4; k++) w[i + k] = u.w[k];
+        }
+        put(i, u.w);
+    }
+    // from, to: what may be read, the memory between the first row's start and the last one's end (a piece that a row's end cuts is read whole where
+    // it lies in it)
+    __device__ __forceinline__ void ask(const T *row, int c, int cols, const T *from, const T *to)
+    {
+        if constexpr(KIND == ROW_WHOLE) {
+            if(c < cols) {
+                #pragma unroll
+                for(int i = 0; i < WORDS<T>; i += 4) put(i, ld_plain(reinterpret_cast<const uint4 *>(row + c) + i / 4));
+            }
+            else {
+                #pragma unroll
+                for(int i = 0; i < WORDS<T>; i += 4) put(i, make_uint4(0, 0, 0, 0));
+            }
+        }
+        else {
+            const int m = off_boundary(row), first = c - lane() * 8;
+            if(row + first - m >= from && row + first - m + WIDTH * 8 + PIECE<T> <= to) {
+                const uint4 *p = reinterpret_cast<const uint4 *>(row + c - m);
+                if(c - m < cols) {
+                    #pragma unroll
+                    for(int i = 0; i < WORDS<T>; i += 4) put(i, ld_plain(p + i / 4));
+                }
+                if(lane() == WIDTH - 1 && c - m + 8 < cols) put(WORDS<T>, ld_plain(p + WORDS<T> / 4));
+            }
+            else {
+                #pragma unroll
+                for(int i = 0; i < WORDS<T>; i += 4) cut_piece(i, row, c - m + i / 4 * PIECE<T>, cols);
+                if(lane() == WIDTH - 1) cut_piece(WORDS<T>, row, c - m + 8, cols);
+            }
         }
     }
-    // the eight elements; all lanes take part
-    __device__ __forceinline__ void settle(const T *row, float (&v)[8])
+    // the eight elements, zeros beyond the row's end; all lanes take part
+    __device__ __forceinline__ void settle(const T *row, int c, int cols, float (&v)[8])
     {
-        if constexpr(OFF) {
+        if constexpr(KIND == ROW_ANY) {
             const int m = off_boundary(row);
             #pragma unroll
             for(int i = 0; i < 4; i++) {
@@ -92,6 +136,10 @@ template<typename T, bool OFF, int WIDTH = 32> struct Row8 {
         for(int i = 0; i < WORDS<T>; i++) u.w[i] = w[i];
         #pragma unroll
         for(int j = 0; j < 8; j++) v[j] = to_float(u.e[j]);
+        if(KIND == ROW_ANY && c + 8 > cols) {
+            #pragma unroll
+            for(int j = 0; j < 8; j++) v[j] = c + j < cols ? v[j] : 0.0f;
+        }
     }
 };
 
@@ -105,13 +153,6 @@ template<typename T> __device__ __forceinline__ void store_piece(T *row, int e, 
         #pragma unroll
         for(int i = 0; i < PIECE<T>; i++)
             if(e + i >= from && e + i < cols) row[e + i] = u.e[i];
-    }
-}
-template<typename T> __device__ __forceinline__ void store_words(T *row, int c, int cols, const uint32_t (&w)[WORDS<T>])
-{
-    if(c < cols) {
-        #pragma unroll
-        for(int g = 0; g < WORDS<T> / 4; g++) store_piece(row, c + g * PIECE<T>, 0, cols, w + g * 4);
     }
 }
 template<typename T> __device__ __forceinline__ void store_words_off(T *row, int c, int cols, const uint32_t (&w)[WORDS<T>])
@@ -135,14 +176,23 @@ template<typename T> __device__ __forceinline__ void store_words_off(T *row, int
             if(i >= PIECE<T> - m && c + 8 - PIECE<T> + i < cols) row[c + 8 - PIECE<T> + i] = u.e[i];
     }
 }
-// OFF: the row may start off a 16-byte boundary
-template<typename T, bool OFF> __device__ __forceinline__ void store8(T *row, int c, int cols, const float (&v)[8])
+template<typename T, int KIND> __device__ __forceinline__ void store8(T *row, int c, int cols, const float (&v)[8])
 {
     union { uint32_t w[WORDS<T>]; T e[8]; } u;
     #pragma unroll
     for(int j = 0; j < 8; j++) u.e[j] = from_float<T>(v[j]);
-    if(OFF && off_boundary(row) != 0) store_words_off(row, c, cols, u.w);
-    else store_words(row, c, cols, u.w);
+    if constexpr(KIND == ROW_WHOLE) {
+        if(c < cols) {
+            #pragma unroll
+            for(int g = 0; g < WORDS<T> / 4; g++)
+                reinterpret_cast<uint4 *>(row + c)[g] = make_uint4(u.w[4 * g], u.w[4 * g + 1], u.w[4 * g + 2], u.w[4 * g + 3]);
+        }
+    }
+    else if(off_boundary(row) != 0) store_words_off(row, c, cols, u.w);
+    else {
+        #pragma unroll
+        for(int g = 0; g < WORDS<T> / 4; g++) store_piece(row, c + g * PIECE<T>, 0, cols, u.w + g * 4);
+    }
 }
 
 // The 8-bit form of a block of values v is a scale s = max|v| / 448 (448: the largest e4m3) and the numbers e4m3(v / s): the largest value
@@ -151,9 +201,9 @@ template<typename T, bool OFF> __device__ __forceinline__ void store8(T *row, in
 // Largest magnitude of the thread's values, as bits (magnitudes are ordered as their bits are); a NaN if one of them is.
 __device__ __forceinline__ unsigned magnitude_bits(const float (&v)[8])
 {
-    float m = fabsf(v[0]);
+    float m = 0.0f;
     #pragma unroll
-    for(int j = 1; j < 8; j++) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v[j])));
+    for(int j = 0; j < 8; j += 2) asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(v[j]), "f"(v[j + 1]));
     return __float_as_uint(m);
 }
 // The quotient by 448 is the product with its reciprocal, corrected by the remainder: rounded as a division would, without its length.
@@ -168,30 +218,25 @@ __device__ __forceinline__ float block_scale(unsigned magnitude)
 __device__ __forceinline__ uint2 pack_e4m3(const float (&v)[8], float scale)
 {
     // (an infinite scale takes the correction out: finite values give 0, infinite ones and NaN a NaN)
-    const float back = scale < __int_as_float(0x7f800000) ? -scale : 0.0f;
+    const Pair back = both(scale < __int_as_float(0x7f800000) ? -scale : 0.0f);
     float inverse;
     asm("rcp.approx.f32 %0, %1;" : "=f"(inverse) : "f"(scale));
-    uint32_t w[2];
+    const Pair inv = both(inverse);
+    unsigned short part[4];
     #pragma unroll
-    for(int i = 0; i < 2; i++) {
-        float q[4];
-        #pragma unroll
-        for(int j = 0; j < 4; j++) {
-            const float q0 = v[4 * i + j] * inverse;
-            q[j] = fmaf(fmaf(back, q0, v[4 * i + j]), inverse, q0);
-        }
-        unsigned short a, b;
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(a) : "f"(q[1]), "f"(q[0]));
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b) : "f"(q[3]), "f"(q[2]));
-        w[i] = uint32_t(a) | uint32_t(b) << 16;
+    for(int i = 0; i < 4; i++) {
+        const Pair x = pair(v[2 * i], v[2 * i + 1]), q0 = x * inv;
+        float lo, hi;
+        apart(fma2(fma2(back, q0, x), inv, q0), lo, hi);
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(part[i]) : "f"(hi), "f"(lo));
     }
-    return make_uint2(w[0], w[1]);
+    return make_uint2(uint32_t(part[0]) | uint32_t(part[1]) << 16, uint32_t(part[2]) | uint32_t(part[3]) << 16);
 }
-// aligned: the row is on an 8-byte boundary
-__device__ __forceinline__ void store_e4m3(unsigned char *row, int c, int cols, bool aligned, uint2 w)
+// The row is on an 8-byte boundary and a multiple of eight long (ROW_WHOLE), or anything.
+template<int KIND> __device__ __forceinline__ void store_e4m3(unsigned char *row, int c, int cols, uint2 w)
 {
-    if(aligned && c + 8 <= cols) *reinterpret_cast<uint2 *>(row + c) = w;
-    else {
+    if(KIND == ROW_WHOLE ? c < cols : (reinterpret_cast<uintptr_t>(row) % 8 == 0 && c + 8 <= cols)) *reinterpret_cast<uint2 *>(row + c) = w;
+    else if(KIND != ROW_WHOLE) {
         #pragma unroll
         for(int j = 0; j < 8; j++)
             if(c + j < cols) row[c + j] = (unsigned char)((j < 4 ? w.x : w.y) >> (8 * (j & 3)));

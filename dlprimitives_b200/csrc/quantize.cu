@@ -6,7 +6,7 @@ namespace dlp {
 namespace {
 
 struct QuantArgs {
-    const void *x;
+    const void *x, *x_end;      // x_end: behind the last row
     unsigned char *q;
     float *scales;
     long long x_stride, q_stride, scale_stride;
@@ -16,89 +16,95 @@ struct QuantArgs {
 // silu(a) = a / (1 + e^-a);  gelu(a) = a / 2 (1 + tanh z) = a / (1 + e^-2z), z = sqrt(2 / pi) (a + 0.044715 a^3): no difference of nearly equal numbers
 // where tanh is near -1.  The quotient is a product with the approximate reciprocal (within a unit): with the division, 8192 x 12288 pairs
 // took longer for their arithmetic than for memory.  Where the exponential overflows the reciprocal is 0.
-__device__ __forceinline__ float gated(float a, float up, int gate)
+// e^-t is 2^s with s = -t log2(e) rounded, and what the rounding (and log2(e) in 24 bits) left out goes in as a factor 1 + left ln 2.  Past |t| = 200
+// nothing changes any more.
+__device__ __forceinline__ void gated2(float &a0, float &a1, float up0, float up1, int gate)
 {
-    const float t = gate == DLP_GATE_SILU ? a : 1.5957691216f * fmaf(0.044715f * a * a, a, a);
-    float r;
-    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.0f + expf(-t)));
-    return a * r * up;
+    const Pair a = pair(a0, a1);
+    float t0 = a0, t1 = a1, s0, s1, e0, e1, r0, r1;
+    if(gate == DLP_GATE_GELU) apart(both(1.5957691216f) * fma2(both(0.044715f) * a * a, a, a), t0, t1);
+    const Pair t = pair(fminf(fmaxf(t0, -200.0f), 200.0f), fminf(fmaxf(t1, -200.0f), 200.0f));
+    const Pair s = t * both(-1.44269502f), left = fma2(t, both(-1.92596299e-8f), fma2(t, both(-1.44269502f), s * both(-1.0f)));
+    apart(s, s0, s1);
+    asm("ex2.approx.f32 %0, %1;" : "=f"(e0) : "f"(s0));
+    asm("ex2.approx.f32 %0, %1;" : "=f"(e1) : "f"(s1));
+    apart(fma2(pair(e0, e1), fma2(left, both(0.693147181f), both(1.0f)), both(1.0f)), e0, e1);
+    asm("rcp.approx.f32 %0, %1;" : "=f"(r0) : "f"(e0));
+    asm("rcp.approx.f32 %0, %1;" : "=f"(r1) : "f"(e1));
+    apart(a * pair(r0, r1) * pair(up0, up1), a0, a1);
 }
 
-constexpr int ROW_THREADS = 256;
+constexpr int ROW_THREADS = 256, ROW_WARPS = ROW_THREADS / 32, ROW_PIECES = 2;
 
-// A warp takes NP pieces of 256 columns of a row, eight a lane of each; sixteen lanes hold a block.  All its loads are under way before the first is
-// used.  OFF: rows start off 16-byte boundaries.
-template<typename T, bool GATED, bool OFF>
-__global__ void __launch_bounds__(ROW_THREADS) quantize_rows_kernel(const QuantArgs a, unsigned groups, unsigned items)
+// A warp takes ROW_PIECES pieces of 256 columns of a row, eight columns a lane of each; sixteen lanes hold a block.  All its loads are under way before the
+// first is used.  2^per_row_log2: warps of a block that share a row; blockIdx.y: blocks that do; KIND: see Row8.  (Blocks that stay, go from row to
+// row and have the next pieces' loads under way were slower, 139 against 121 us for 8192 x 12288 pairs: a block that ends makes room for one that
+// starts with its loads, which keeps memory busy under the others' arithmetic better than a fixed order within each warp.)
+template<typename T, bool GATED, int KIND>
+__global__ void __launch_bounds__(ROW_THREADS, 4) quantize_rows_kernel(const QuantArgs a, int per_row_log2)
 {
     pdl_wait();
-    constexpr int NP = GATED || sizeof(T) == 4 ? 2 : 4;
-    const int lane = threadIdx.x & 31, cols = a.cols;
-    const unsigned step = gridDim.x * (ROW_THREADS / 32);
-    for(unsigned item = blockIdx.x * (ROW_THREADS / 32) + (threadIdx.x >> 5); item < items; item += step) {
-        const unsigned row = item / groups;
-        const int c0 = int(item - row * groups) * (256 * NP) + lane * 8;
-        const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
-        Row8<T, OFF> w[NP], u[GATED ? NP : 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cols = a.cols, per_row = 1 << per_row_log2;
+    const long long row = (long long)blockIdx.x * (ROW_WARPS >> per_row_log2) + (warp >> per_row_log2);
+    if(row >= a.rows) return;
+    const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
+    const T *from = static_cast<const T *>(a.x), *to = static_cast<const T *>(a.x_end);
+    unsigned char *q = a.q + row * a.q_stride;
+    float *scale = a.scales + row;
+    const int step = gridDim.y * per_row * (256 * ROW_PIECES);
+    #pragma unroll 1
+    for(int c0 = (blockIdx.y * per_row + (warp & (per_row - 1))) * (256 * ROW_PIECES) + lane * 8; c0 - lane * 8 < cols; c0 += step) {
+        Row8<T, KIND> w[ROW_PIECES], u[GATED ? ROW_PIECES : 1];
         #pragma unroll
-        for(int i = 0; i < NP; i++) {
-            w[i].ask(x, c0 + i * 256, cols);
-            if(GATED) u[GATED ? i : 0].ask(x + cols, c0 + i * 256, cols);
+        for(int i = 0; i < ROW_PIECES; i++) {
+            w[i].ask(x, c0 + i * 256, cols, from, to);
+            if(GATED) u[GATED ? i : 0].ask(x + cols, c0 + i * 256, cols, from, to);
         }
         #pragma unroll
-        for(int i = 0; i < NP; i++) {
-            w[i].patch(x, c0 + i * 256, cols);
-            if(GATED) u[GATED ? i : 0].patch(x + cols, c0 + i * 256, cols);
-        }
-        unsigned char *q = a.q + row * a.q_stride;
-        const bool aligned = reinterpret_cast<uintptr_t>(q) % 8 == 0;
-        #pragma unroll
-        for(int i = 0; i < NP; i++) {
+        for(int i = 0; i < ROW_PIECES; i++) {
             const int c = c0 + i * 256;
             float v[8];
-            w[i].settle(x, v);
+            w[i].settle(x, c, cols, v);
             if(GATED) {
                 float up[8];
-                u[GATED ? i : 0].settle(x + cols, up);
+                u[GATED ? i : 0].settle(x + cols, c, cols, up);
                 if(a.gate == DLP_GATE_SILU) {
                     #pragma unroll
-                    for(int j = 0; j < 8; j++) v[j] = gated(v[j], up[j], DLP_GATE_SILU);
+                    for(int j = 0; j < 8; j += 2) gated2(v[j], v[j + 1], up[j], up[j + 1], DLP_GATE_SILU);
                 }
                 else {
                     #pragma unroll
-                    for(int j = 0; j < 8; j++) v[j] = gated(v[j], up[j], DLP_GATE_GELU);
+                    for(int j = 0; j < 8; j += 2) gated2(v[j], v[j + 1], up[j], up[j + 1], DLP_GATE_GELU);
                 }
             }
             const float s = block_scale(__reduce_max_sync(lane < 16 ? 0xffffu : 0xffff0000u, magnitude_bits(v)));
-            if((lane & 15) == 0 && c < cols) a.scales[(c / SCALE_BLOCK) * a.scale_stride + row] = s;
-            store_e4m3(q, c, cols, aligned, pack_e4m3(v, s));
+            if((lane & 15) == 0 && c < cols) scale[(c / SCALE_BLOCK) * a.scale_stride] = s;
+            store_e4m3<KIND>(q, c, cols, pack_e4m3(v, s));
         }
     }
 }
 
 // A block of 256 threads takes a block of 128 x 128 and keeps it in registers: sixteen lanes hold a row, a thread eight rows.
-template<typename T, bool OFF>
+template<typename T, int KIND>
 __global__ void __launch_bounds__(256) quantize_blocks_kernel(const QuantArgs a)
 {
     pdl_wait();
     __shared__ unsigned most[8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int c = blockIdx.x * SCALE_BLOCK + (lane & 15) * 8, row0 = blockIdx.y * SCALE_BLOCK + warp * 2 + (lane >> 4);
-    Row8<T, OFF, 16> w[8];
+    Row8<T, KIND, 16> w[8];
     const T *x[8];
     const auto cols_of = [&](int i) { return row0 + i * 16 < a.rows ? a.cols : 0; };       // a row that is not there has no columns
     #pragma unroll
     for(int i = 0; i < 8; i++) {
         x[i] = static_cast<const T *>(a.x) + (row0 + i * 16 < a.rows ? row0 + i * 16 : 0) * a.x_stride;
-        w[i].ask(x[i], c, cols_of(i));
+        w[i].ask(x[i], c, cols_of(i), static_cast<const T *>(a.x), static_cast<const T *>(a.x_end));
     }
-    #pragma unroll
-    for(int i = 0; i < 8; i++) w[i].patch(x[i], c, cols_of(i));
     float v[8][8];
     unsigned m = 0;
     #pragma unroll
     for(int i = 0; i < 8; i++) {
-        w[i].settle(x[i], v[i]);
+        w[i].settle(x[i], c, cols_of(i), v[i]);
         m = max(m, magnitude_bits(v[i]));
     }
     m = __reduce_max_sync(0xffffffffu, m);
@@ -113,20 +119,23 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const QuantArgs a)
         const int row = row0 + i * 16;
         const uint2 q = pack_e4m3(v[i], s);
         unsigned char *to = a.q + (row < a.rows ? row : 0) * a.q_stride;
-        if(row < a.rows) store_e4m3(to, c, a.cols, reinterpret_cast<uintptr_t>(to) % 8 == 0, q);
+        if(row < a.rows) store_e4m3<KIND>(to, c, a.cols, q);
     }
 }
 
 template<typename T, bool GATED>
 dlp_status launch_rows(const QuantArgs &a, bool off, cudaStream_t stream)
 {
-    const int groups = ceil_div(a.cols, 256 * (GATED || sizeof(T) == 4 ? 2 : 4));
-    const long long items = (long long)a.rows * groups, blocks = ceil_div<long long>(items, ROW_THREADS / 32);
-    DLP_REQUIRE(items < (1ll << 32) - (1 << 24), "too many rows");
-    const unsigned grid = unsigned(std::min<long long>(blocks, (long long)sm_count() * 64));
-    const bool early = one_wave(grid, ROW_THREADS);
-    if(off) DLP_LAUNCH_PDL(launch_pdl(early, quantize_rows_kernel<T, GATED, true>, grid, ROW_THREADS, 0, stream, a, unsigned(groups), unsigned(items)), "quantize_rows_kernel");
-    else DLP_LAUNCH_PDL(launch_pdl(early, quantize_rows_kernel<T, GATED, false>, grid, ROW_THREADS, 0, stream, a, unsigned(groups), unsigned(items)), "quantize_rows_kernel");
+    const int groups = ceil_div(a.cols, 256 * ROW_PIECES);
+    int log2 = 0;
+    while((1 << log2) < std::min(groups, ROW_WARPS)) log2++;
+    const int blocks = ceil_div(a.rows, ROW_WARPS >> log2);
+    // few rows: more blocks to a row, until the GPU is full
+    const int across = std::max(1, std::min(ceil_div(groups, 1 << log2), sm_count() * 4 / blocks));
+    const dim3 grid(blocks, across);
+    const bool early = one_wave((long long)blocks * across, ROW_THREADS);
+    if(off) DLP_LAUNCH_PDL(launch_pdl(early, quantize_rows_kernel<T, GATED, ROW_ANY>, grid, ROW_THREADS, 0, stream, a, log2), "quantize_rows_kernel");
+    else DLP_LAUNCH_PDL(launch_pdl(early, quantize_rows_kernel<T, GATED, ROW_WHOLE>, grid, ROW_THREADS, 0, stream, a, log2), "quantize_rows_kernel");
     return DLP_OK;
 }
 template<typename T>
@@ -135,8 +144,8 @@ dlp_status launch_quantize(const QuantArgs &a, int block_rows, bool off, cudaStr
     if(block_rows == 1) return a.gate == DLP_GATE_NONE ? launch_rows<T, false>(a, off, stream) : launch_rows<T, true>(a, off, stream);
     const dim3 grid(ceil_div(a.cols, SCALE_BLOCK), ceil_div(a.rows, SCALE_BLOCK));
     const bool early = one_wave((long long)grid.x * grid.y, 256);
-    if(off) DLP_LAUNCH_PDL(launch_pdl(early, quantize_blocks_kernel<T, true>, grid, 256, 0, stream, a), "quantize_blocks_kernel");
-    else DLP_LAUNCH_PDL(launch_pdl(early, quantize_blocks_kernel<T, false>, grid, 256, 0, stream, a), "quantize_blocks_kernel");
+    if(off) DLP_LAUNCH_PDL(launch_pdl(early, quantize_blocks_kernel<T, ROW_ANY>, grid, 256, 0, stream, a), "quantize_blocks_kernel");
+    else DLP_LAUNCH_PDL(launch_pdl(early, quantize_blocks_kernel<T, ROW_WHOLE>, grid, 256, 0, stream, a), "quantize_blocks_kernel");
     return DLP_OK;
 }
 
@@ -164,9 +173,10 @@ dlp_status dlp_quantize_fwd(const dlp_quantize_args *args, void *stream)
     DLP_REQUIRE(block_rows == 1 || rows <= 65535 * SCALE_BLOCK, "too many rows");
     const size_t size = type_size(type);
     DLP_REQUIRE(aligned_to(x, size) && aligned_to(scales, 4), "a tensor is not aligned to its elements");
-    const QuantArgs a = { x, static_cast<unsigned char *>(q), scales, x_stride, q_stride, scale_stride, rows, cols, gate };
-    // every row, and the second half of a pair's, on a 16-byte boundary?
-    const bool off = !(aligned_to(x, 16) && (rows == 1 || x_stride * size % 16 == 0) && (gate == DLP_GATE_NONE || cols * size % 16 == 0));
+    const long long length = (rows - 1) * (rows > 1 ? x_stride : 0) + (gate == DLP_GATE_NONE ? 1ll : 2ll) * cols;
+    const QuantArgs a = { x, static_cast<const char *>(x) + length * (long long)size, static_cast<unsigned char *>(q), scales, x_stride, q_stride, scale_stride, rows, cols, gate };
+    // every row, and the second half of a pair's, on a 16-byte boundary (8 for the numbers) and a multiple of eight long?
+    const bool off = !(cols % 8 == 0 && aligned_to(x, 16) && aligned_to(q, 8) && (rows == 1 || (x_stride * size % 16 == 0 && q_stride % 8 == 0)));
     if(type == DLP_TYPE_F32) return launch_quantize<float>(a, block_rows, off, (cudaStream_t)stream);
     if(type == DLP_TYPE_F16) return launch_quantize<__half>(a, block_rows, off, (cudaStream_t)stream);
     return launch_quantize<__nv_bfloat16>(a, block_rows, off, (cudaStream_t)stream);

@@ -9,7 +9,7 @@ namespace dlp {
 namespace {
 
 struct NormArgs {
-    const void *x, *residual, *weight;
+    const void *x, *residual, *weight, *x_end, *residual_end, *weight_end;       // .._end: behind the last row
     void *total, *y;
     float *scales;
     long long x_stride, residual_stride, total_stride, y_stride, scale_stride;
@@ -41,35 +41,35 @@ __device__ __forceinline__ float inverse_root(float v)
 }
 
 // What becomes of eight values h of a row: total, and the output in its type.
-template<typename T, bool OFF>
+template<typename T, int KIND>
 __device__ __forceinline__ void norm_out(const NormArgs &a, long long row, int c, float (&v)[8], const float (&g)[8], float f)
 {
     const int lane = threadIdx.x & 31;
-    if(a.total) store8<T, OFF>(static_cast<T *>(a.total) + row * a.total_stride, c, a.cols, v);
+    if(a.total) store8<T, KIND>(static_cast<T *>(a.total) + row * a.total_stride, c, a.cols, v);
     #pragma unroll
-    for(int j = 0; j < 8; j++) v[j] = v[j] * f * g[j];
+    for(int j = 0; j < 8; j += 2) apart(pair(v[j], v[j + 1]) * both(f) * pair(g[j], g[j + 1]), v[j], v[j + 1]);
     if(a.y_type == DLP_TYPE_E4M3) {
         const float s = block_scale(__reduce_max_sync(lane < 16 ? 0xffffu : 0xffff0000u, magnitude_bits(v)));
         unsigned char *y = static_cast<unsigned char *>(a.y) + row * a.y_stride;
         if((lane & 15) == 0 && c < a.cols) a.scales[(c / SCALE_BLOCK) * a.scale_stride + row] = s;
-        store_e4m3(y, c, a.cols, reinterpret_cast<uintptr_t>(y) % 8 == 0, pack_e4m3(v, s));
+        store_e4m3<KIND>(y, c, a.cols, pack_e4m3(v, s));
     }
-    else if(a.y_type == DLP_TYPE_F32) store8<float, OFF>(static_cast<float *>(a.y) + row * a.y_stride, c, a.cols, v);
-    else if(a.y_type == DLP_TYPE_F16) store8<__half, OFF>(static_cast<__half *>(a.y) + row * a.y_stride, c, a.cols, v);
-    else store8<__nv_bfloat16, OFF>(static_cast<__nv_bfloat16 *>(a.y) + row * a.y_stride, c, a.cols, v);
+    else if(a.y_type == DLP_TYPE_F32) store8<float, KIND>(static_cast<float *>(a.y) + row * a.y_stride, c, a.cols, v);
+    else if(a.y_type == DLP_TYPE_F16) store8<__half, KIND>(static_cast<__half *>(a.y) + row * a.y_stride, c, a.cols, v);
+    else store8<__nv_bfloat16, KIND>(static_cast<__nv_bfloat16 *>(a.y) + row * a.y_stride, c, a.cols, v);
 }
 
-constexpr bool half_registers(int nv, bool off) { return nv <= 2 && !off; }
+constexpr bool half_registers(int nv, int kind) { return nv <= 2 && kind == ROW_WHOLE; }
 
 // NV: pieces of eight columns that a thread keeps, a block's width apart, so that a warp has 256 consecutive columns, two blocks of the 8-bit form.
-// OFF: rows of some tensor start off 16-byte boundaries.  A block takes rows in turn and asks for the next one as soon as the registers of this one's
+// KIND: see Row8, of all tensors together.  A block takes rows in turn and asks for the next one as soon as the registers of this one's
 // words are free: the reduction, the arithmetic and the stores of a row run under the loads of the next.  The weights stay.
-template<typename T, int NV, bool OFF>
-__global__ void __launch_bounds__(MAX_THREADS, half_registers(NV, OFF) ? 2 : 1) rms_norm_kernel(const NormArgs a, int rows)
+template<typename T, int NV, int KIND>
+__global__ void __launch_bounds__(MAX_THREADS, half_registers(NV, KIND) ? 2 : 1) rms_norm_kernel(const NormArgs a, int rows)
 {
     pdl_wait();
     __shared__ float part[2][MAX_THREADS / 32];
-    typedef Row8<T, OFF> Row;
+    typedef Row8<T, KIND> Row;
     const int cols = a.cols, stride = blockDim.x * 8, c0 = threadIdx.x * 8;
     const T *weight = static_cast<const T *>(a.weight);
     const auto x_at = [&](long long row) { return static_cast<const T *>(a.x) + row * a.x_stride; };
@@ -79,38 +79,35 @@ __global__ void __launch_bounds__(MAX_THREADS, half_registers(NV, OFF) ? 2 : 1) 
     auto ask = [&](long long row) {
         #pragma unroll
         for(int i = 0; i < NV; i++) {
-            xw[i].ask(x_at(row), c0 + i * stride, cols);
-            if(a.residual) rw[i].ask(r_at(row), c0 + i * stride, cols);
+            xw[i].ask(x_at(row), c0 + i * stride, cols, x_at(0), static_cast<const T *>(a.x_end));
+            if(a.residual) rw[i].ask(r_at(row), c0 + i * stride, cols, r_at(0), static_cast<const T *>(a.residual_end));
         }
     };
     ask(blockIdx.x);
     if(KEEP_WEIGHT) {
         #pragma unroll
-        for(int i = 0; i < NV; i++) ww[KEEP_WEIGHT ? i : 0].ask(weight, c0 + i * stride, cols);
-        #pragma unroll
-        for(int i = 0; i < NV; i++) ww[KEEP_WEIGHT ? i : 0].patch(weight, c0 + i * stride, cols);
+        for(int i = 0; i < NV; i++) ww[KEEP_WEIGHT ? i : 0].ask(weight, c0 + i * stride, cols, weight, static_cast<const T *>(a.weight_end));
     }
     int turn = 0;
     #pragma unroll 1
     for(int row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
-        float h[NV][8], sum = 0.0f;
+        float h[NV][8];
+        Pair squares = both(0.0f);
         #pragma unroll
         for(int i = 0; i < NV; i++) {
-            xw[i].patch(x_at(row), c0 + i * stride, cols);
-            if(a.residual) rw[i].patch(r_at(row), c0 + i * stride, cols);
-        }
-        #pragma unroll
-        for(int i = 0; i < NV; i++) {
-            xw[i].settle(x_at(row), h[i]);
+            xw[i].settle(x_at(row), c0 + i * stride, cols, h[i]);
             if(a.residual) {
                 float b[8];
-                rw[i].settle(r_at(row), b);
+                rw[i].settle(r_at(row), c0 + i * stride, cols, b);
                 #pragma unroll
-                for(int j = 0; j < 8; j++) h[i][j] += b[j];
+                for(int j = 0; j < 8; j += 2) apart(pair(h[i][j], h[i][j + 1]) + pair(b[j], b[j + 1]), h[i][j], h[i][j + 1]);
             }
             #pragma unroll
-            for(int j = 0; j < 8; j++) sum += h[i][j] * h[i][j];
+            for(int j = 0; j < 8; j += 2) squares = fma2(pair(h[i][j], h[i][j + 1]), pair(h[i][j], h[i][j + 1]), squares);
         }
+        float sum, odd;
+        apart(squares, sum, odd);
+        sum += odd;
         if(row + int(gridDim.x) < rows) ask(row + int(gridDim.x));
         const float f = inverse_root(block_sum(sum, part[turn]) / float(cols) + a.eps);
         #pragma unroll
@@ -118,19 +115,16 @@ __global__ void __launch_bounds__(MAX_THREADS, half_registers(NV, OFF) ? 2 : 1) 
             const int c = c0 + i * stride;
             Row w;
             if(KEEP_WEIGHT) w = ww[KEEP_WEIGHT ? i : 0];
-            else {
-                w.ask(weight, c, cols);
-                w.patch(weight, c, cols);
-            }
+            else w.ask(weight, c, cols, weight, static_cast<const T *>(a.weight_end));
             float g[8];
-            w.settle(weight, g);
-            norm_out<T, OFF>(a, row, c, h[i], g, f);
+            w.settle(weight, c, cols, g);
+            norm_out<T, KIND>(a, row, c, h[i], g, f);
         }
     }
 }
 
 // Rows of more than a block's registers: read twice, the second time from L2.
-template<typename T, bool OFF>
+template<typename T, int KIND>
 __global__ void __launch_bounds__(MAX_THREADS, 2) rms_norm_long_kernel(const NormArgs a)
 {
     pdl_wait();
@@ -140,15 +134,13 @@ __global__ void __launch_bounds__(MAX_THREADS, 2) rms_norm_long_kernel(const Nor
     const T *x = static_cast<const T *>(a.x) + row * a.x_stride, *weight = static_cast<const T *>(a.weight);
     const T *r = a.residual ? static_cast<const T *>(a.residual) + row * a.residual_stride : nullptr;
     auto fetch = [&](int c, float (&h)[8]) {
-        Row8<T, OFF> xw, rw;
-        xw.ask(x, c, cols);
-        if(r) rw.ask(r, c, cols);
-        xw.patch(x, c, cols);
-        xw.settle(x, h);
+        Row8<T, KIND> xw, rw;
+        xw.ask(x, c, cols, static_cast<const T *>(a.x), static_cast<const T *>(a.x_end));
+        if(r) rw.ask(r, c, cols, static_cast<const T *>(a.residual), static_cast<const T *>(a.residual_end));
+        xw.settle(x, c, cols, h);
         if(r) {
             float b[8];
-            rw.patch(r, c, cols);
-            rw.settle(r, b);
+            rw.settle(r, c, cols, b);
             #pragma unroll
             for(int j = 0; j < 8; j++) h[j] += b[j];
         }
@@ -164,21 +156,20 @@ __global__ void __launch_bounds__(MAX_THREADS, 2) rms_norm_long_kernel(const Nor
     for(int c0 = 0; c0 < cols; c0 += stride) {
         const int c = c0 + threadIdx.x * 8;
         float h[8], g[8];
-        Row8<T, OFF> w;
-        w.ask(weight, c, cols);
+        Row8<T, KIND> w;
+        w.ask(weight, c, cols, weight, static_cast<const T *>(a.weight_end));
         fetch(c, h);
-        w.patch(weight, c, cols);
-        w.settle(weight, g);
-        norm_out<T, OFF>(a, row, c, h, g, f);
+        w.settle(weight, c, cols, g);
+        norm_out<T, KIND>(a, row, c, h, g, f);
     }
 }
 
 template<typename T, int NV>
 dlp_status launch_nv(const NormArgs &a, int rows, int threads, bool off, cudaStream_t stream)
 {
-    const int blocks = std::min(rows, sm_count() * std::max(1, (half_registers(NV, off) ? 1024 : 512) / threads));       // all of them resident
-    if(off) DLP_LAUNCH_PDL(launch_pdl(true, rms_norm_kernel<T, NV, true>, blocks, threads, 0, stream, a, rows), "rms_norm_kernel");
-    else DLP_LAUNCH_PDL(launch_pdl(true, rms_norm_kernel<T, NV, false>, blocks, threads, 0, stream, a, rows), "rms_norm_kernel");
+    const int blocks = std::min(rows, sm_count() * std::max(1, (half_registers(NV, off ? ROW_ANY : ROW_WHOLE) ? 1024 : 512) / threads));       // all of them resident
+    if(off) DLP_LAUNCH_PDL(launch_pdl(true, rms_norm_kernel<T, NV, ROW_ANY>, blocks, threads, 0, stream, a, rows), "rms_norm_kernel");
+    else DLP_LAUNCH_PDL(launch_pdl(true, rms_norm_kernel<T, NV, ROW_WHOLE>, blocks, threads, 0, stream, a, rows), "rms_norm_kernel");
     return DLP_OK;
 }
 template<typename T>
@@ -191,8 +182,8 @@ dlp_status launch_norm(const NormArgs &a, int rows, bool off, cudaStream_t strea
     const int threads = round_up(ceil_div(pieces, nv), 32);
     if(threads > MAX_THREADS) {
         const bool early = one_wave(rows, MAX_THREADS);
-        if(off) DLP_LAUNCH_PDL(launch_pdl(early, rms_norm_long_kernel<T, true>, rows, MAX_THREADS, 0, stream, a), "rms_norm_long_kernel");
-        else DLP_LAUNCH_PDL(launch_pdl(early, rms_norm_long_kernel<T, false>, rows, MAX_THREADS, 0, stream, a), "rms_norm_long_kernel");
+        if(off) DLP_LAUNCH_PDL(launch_pdl(early, rms_norm_long_kernel<T, ROW_ANY>, rows, MAX_THREADS, 0, stream, a), "rms_norm_long_kernel");
+        else DLP_LAUNCH_PDL(launch_pdl(early, rms_norm_long_kernel<T, ROW_WHOLE>, rows, MAX_THREADS, 0, stream, a), "rms_norm_long_kernel");
         return DLP_OK;
     }
     switch(nv) {
@@ -228,10 +219,13 @@ dlp_status dlp_rms_norm_fwd(const dlp_rms_norm_args *args, void *stream)
     const size_t size = type_size(type), y_size = type_size(y_type);
     DLP_REQUIRE(aligned_to(x, size) && aligned_to(weight, size) && aligned_to(y, y_size) && (!residual || aligned_to(residual, size)) &&
                 (!total || aligned_to(total, size)) && (!scales || aligned_to(scales, 4)), "a tensor is not aligned to its elements");
-    NormArgs a = { x, residual, weight, total, y, scales, x_stride, residual_stride, total_stride, y_stride, scale_stride, cols, y_type, eps };
-    const auto rows_on = [rows = args->rows](const void *p, long long stride, size_t element) { return aligned_to(p, 16) && (rows == 1 || stride * element % 16 == 0); };
-    const bool off = !(rows_on(x, x_stride, size) && aligned_to(weight, 16) && (!residual || rows_on(residual, residual_stride, size)) &&
-                       (!total || rows_on(total, total_stride, size)) && (y_type == DLP_TYPE_E4M3 || rows_on(y, y_stride, y_size)));
+    const auto end = [rows = args->rows, cols = args->cols](const void *p, long long stride, size_t element) -> const void * {
+        return p ? static_cast<const char *>(p) + ((rows - 1) * (rows > 1 ? stride : 0) + cols) * (long long)element : nullptr;
+    };
+    NormArgs a = { x, residual, weight, end(x, x_stride, size), end(residual, residual_stride, size), end(weight, 0, size), total, y, scales, x_stride, residual_stride, total_stride, y_stride, scale_stride, cols, y_type, eps };
+    const auto rows_on = [rows = args->rows](const void *p, long long stride, size_t element, size_t n) { return aligned_to(p, n) && (rows == 1 || stride * element % n == 0); };
+    const bool off = !(cols % 8 == 0 && rows_on(x, x_stride, size, 16) && aligned_to(weight, 16) && (!residual || rows_on(residual, residual_stride, size, 16)) &&
+                       (!total || rows_on(total, total_stride, size, 16)) && rows_on(y, y_stride, y_size, y_type == DLP_TYPE_E4M3 ? 8 : 16));
     if(type == DLP_TYPE_F32) return launch_norm<float>(a, rows, off, (cudaStream_t)stream);
     if(type == DLP_TYPE_F16) return launch_norm<__half>(a, rows, off, (cudaStream_t)stream);
     return launch_norm<__nv_bfloat16>(a, rows, off, (cudaStream_t)stream);
