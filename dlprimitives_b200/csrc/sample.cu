@@ -12,10 +12,10 @@
 // blocks gather what each has found through distributed shared memory and all come to the same conclusions.
 //   * First the largest logit, and the largest of each of 512 groups of classes.
 //   * With a small k (up to 256): the k-th largest of the groups' maxima has at least k classes at or above it, and for classes in no
-//     particular order only a few more (512 ln(512 / (512 - k)) of them are expected).  These are collected, sorted, and the rest is done on
+//     particular order only a few more (512 ln(512 / (512 - k)) of them are expected).  These are collected, and the rest is done on
 //     them alone: two readings of the row, and masses of a few hundred classes.
-//   * Otherwise the end of a prefix is found from sums over 4096 bins of falling logits: the bin it lies in is collected and sorted,
-//     and divided further as long as it holds more than 512 classes.  Then the masses of the kept classes are summed by
+//   * Otherwise the end of a prefix is found from sums over 2048 bins of falling logits: the bin it lies in is collected, and divided
+//     further as long as it holds more than 512 classes.  Then the masses of the kept classes are summed by
 //     segments of the row, and the one segment that the random number points into is gone through.
 #include "block8.cuh"
 
@@ -34,7 +34,7 @@ struct SampleArgs {
 };
 
 constexpr int THREADS = 512, WARPS = THREADS / 32, MAX_PARTS = 8;
-constexpr int BINS = 4096, CAP = THREADS;        // bins of a histogram; classes that are sorted at once
+constexpr int BINS = 2048, CAP = THREADS;        // bins of a histogram; classes that are sorted at once
 constexpr int SMALL_K = 256;
 constexpr unsigned MASKED = 0;                   // the key of -inf and of NaN
 constexpr unsigned LOWEST = 0x00800000u;         // the key of the lowest finite number
@@ -54,15 +54,17 @@ template<> constexpr int grain_bits<__nv_bfloat16> = 16;
 struct Scratch {
     u64 all_mass[BINS];                          // sums over the row's classes,
     unsigned all_count[BINS];
-    unsigned mass_lo[BINS], mass_hi[BINS], count[BINS];     // and over this block's
-    u64 cand[CAP], sorted[2][CAP];               // classes as (key, ~index)
+    uint2 mass[BINS];                            // and over this block's, in two halves
+    unsigned count[BINS];
+    u64 cand[CAP], list[CAP], list_mass[CAP];    // classes as (key, ~index): this block's, and the row's with their masses
+    u64 sorted[2][CAP];
     u64 seg_mass[WARPS];                         // kept masses of each warp's segment, and classes equal to the cut's key
     unsigned seg_ties[WARPS];
     u64 best[WARPS];
     unsigned group[THREADS];
     u64 warp_sum[2][WARPS];
-    u64 found[3];
-    double table[64];                            // 2^(-j / 64)
+    u64 found[3], rest[2];
+    double table[1024];                          // of Masses
     unsigned cands;
 };
 
@@ -86,41 +88,37 @@ __device__ __forceinline__ unsigned peer(const unsigned *p, int rank)
     return v;
 }
 
-// A mass of a class.  w = 2^-t with t = (max - x) log2(e) / temperature, in 64 bits: t = i + j / 64 + r with whole i and j, |r| <= 1/128, and
-// 2^-r by the series of exp(-r ln 2), whose sixth term is under 2^-53.
+// A mass of a class.  w = 2^-t with t = (max - x) log2(e) / temperature, in 64 bits: t = i + j / 1024 + r with whole i and j, |r| <= 1/2048, and
+// 2^-r by the series of exp(-r ln 2), whose fourth term is under 2^-50.
+constexpr int STEPS = 1024;
 struct Masses {
-    double top, factor, one, least;              // factor: log2(e) / temperature; one: 2^bits; least: w of min-p
-    unsigned top_key;
-    const double *table;
-    __device__ __forceinline__ double weight(unsigned key) const
+    double top_t, factor, one, least;            // factor: log2(e) / temperature; top_t: max times that; one: 2^bits; least: w of min-p
+    float top;
+    const double *table;                         // 2^(-j / STEPS)
+    // No branches: a chain of dependent operations, of which several run side by side where several are asked for.
+    __device__ __forceinline__ double weight(float x) const
     {
-        if(key == top_key) return 1.0;
-        const double t = (top - double(value_of(key))) * factor;
-        if(!(t < 1000.0)) return 0.0;            // (and an infinite logit's NaN)
-        const double magic = 6755399441055744.0 / 64.0, z = t + magic, r = t - (z - magic);
-        const int k = __double2loint(z);         // 64 i + j
-        constexpr double L = 0.69314718055994530942, C2 = L * L / 2, C3 = L * C2 / 3, C4 = L * C3 / 4, C5 = L * C4 / 5;
-        const double e = fma(r, fma(r, fma(r, fma(r, fma(r, -C5, C4), -C3), C2), -L), 1.0) * table[k & 63];
-        const int i = k >> 6;
-        return __hiloint2double(__double2hiint(e) - (i << 20), __double2loint(e));      // e is in (0.49, 1.01), i under 1001: the exponent stays normal
+        const double v = double(x), magic = 6755399441055744.0 / STEPS, t = fma(-v, factor, top_t), z = t + magic, r = t - (z - magic);
+        const int k = __double2loint(z);         // STEPS i + j
+        constexpr double L = 0.69314718055994530942, C2 = L * L / 2, C3 = L * C2 / 3;
+        const double e = fma(r, fma(r, fma(r, -C3, C2), -L), 1.0) * table[k & (STEPS - 1)];
+        // for t < 1000: e is in (0.49, 1.01), k / STEPS under 1001, and the exponent stays normal.  (t is infinite or NaN for -inf and NaN, and where the
+        // largest logit is infinite.)
+        const double w = t < 1000.0 ? __hiloint2double(__double2hiint(e) - (k / STEPS << 20), __double2loint(e)) : 0.0;
+        return x == top ? 1.0 : w;
     }
     // a whole number below 2^52 is the low part of itself + 2^52
     __device__ __forceinline__ u64 whole(double w) const { return u64(__double_as_longlong(fma(w, one, 4503599627370496.0)) & 0xfffffffffffffll); }
-    __device__ __forceinline__ u64 mass(unsigned key) const { return key == MASKED ? 0 : whole(weight(key)); }
+    __device__ __forceinline__ u64 mass(float x) const { return whole(weight(x)); }
+    __device__ __forceinline__ u64 mass(unsigned key) const { return mass(value_of(key)); }
 };
 
 // Where a prefix of the sorted row ends: all above `key` and the first `ties` of those equal to it.
 struct Cut { unsigned key, ties; };
 
-// ---- over the first `active` threads (a multiple of 32, THREADS: the whole block), all of which take part
-__device__ __forceinline__ void sync(int active)
-{
-    if(active == THREADS) __syncthreads();
-    else if(active == 32) __syncwarp();
-    else asm volatile("bar.sync 1, %0;" ::"r"(active) : "memory");
-}
+// ---- over the block (every thread takes part)
 // Sum up to and with this thread's value, and of all.  flip: changes from call to call, so that one barrier a call is enough.
-__device__ __forceinline__ u64 scan(u64 v, Scratch &sh, int &flip, u64 &all, int active)
+__device__ __forceinline__ u64 scan(u64 v, Scratch &sh, int &flip, u64 &all)
 {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     #pragma unroll
@@ -128,41 +126,64 @@ __device__ __forceinline__ u64 scan(u64 v, Scratch &sh, int &flip, u64 &all, int
         const u64 other = __shfl_up_sync(0xffffffffu, v, o);
         if(lane >= o) v += other;
     }
-    if(active == 32) {
-        all = __shfl_sync(0xffffffffu, v, 31);
-        return v;
-    }
     flip ^= 1;
     if(lane == 31) sh.warp_sum[flip][warp] = v;
-    sync(active);
-    u64 sums = lane < active / 32 ? sh.warp_sum[flip][lane] : 0;
+    __syncthreads();
+    u64 sums = sh.warp_sum[flip][lane & (WARPS - 1)];
     #pragma unroll
     for(int o = 1; o < WARPS; o <<= 1) {
         const u64 other = __shfl_up_sync(0xffffffffu, sums, o);
-        if(lane >= o) sums += other;
+        if((lane & (WARPS - 1)) >= o) sums += other;
     }
     all = __shfl_sync(0xffffffffu, sums, WARPS - 1);
     const u64 before = __shfl_sync(0xffffffffu, sums, warp > 0 ? warp - 1 : 0);
     return v + (warp > 0 ? before : 0);
 }
-// Sorts the numbers of the first `size` threads (a power of two), the largest first; the others' are zeros.
-__device__ __forceinline__ u64 sort(u64 v, int size, Scratch &sh, int active)
+// Sum over the block; flip: as in scan.
+__device__ __forceinline__ u64 sum_all(u64 v, Scratch &sh, int &flip)
+{
+    const int lane = threadIdx.x & 31;
+    #pragma unroll
+    for(int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    flip ^= 1;
+    if(lane == 0) sh.warp_sum[flip][threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = sh.warp_sum[flip][lane & (WARPS - 1)];
+    #pragma unroll
+    for(int o = WARPS / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// Lists of up to CAP classes in shared memory.  Short ones are gone through, each class against each, by `each` neighbouring threads (a power of two, at
+// most 32) to a class that share the list: f(number, mass) for a thread's share.  Long ones are sorted.
+constexpr int COUNTED = 128;
+template<typename F> __device__ __forceinline__ void through(const Scratch &sh, int total, int each, F f)
+{
+    #pragma unroll 4
+    for(int i = threadIdx.x & (each - 1); i < total; i += each) f(sh.list[i], sh.list_mass[i]);
+}
+__device__ __forceinline__ u64 sum_of(u64 v, int each)       // over the threads that share a class
+{
+    for(int o = 1; o < each; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// Sorts the threads' numbers, the largest first.
+__device__ __forceinline__ u64 sort(u64 v, Scratch &sh)
 {
     const int tid = threadIdx.x;
     int buf = 0;
     #pragma unroll 1
-    for(int k = 2; k <= size; k <<= 1)
+    for(int k = 2; k <= THREADS; k <<= 1)
         #pragma unroll 1
         for(int j = k >> 1; j > 0; j >>= 1) {
             u64 other;
             if(j >= 32) {
                 sh.sorted[buf][tid] = v;
-                sync(active);
+                __syncthreads();
                 other = sh.sorted[buf][tid ^ j];
                 buf ^= 1;
             }
             else other = __shfl_xor_sync(0xffffffffu, v, j);
-            const bool larger = ((tid & j) == 0) == ((tid & k) == 0 || k == size);
+            const bool larger = ((tid & j) == 0) == ((tid & k) == 0 || k == THREADS);
             v = larger == (v > other) ? v : other;
         }
     return v;
@@ -217,25 +238,43 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a)
             }
         }
     };
-    // f(key) for the segment's classes that can be drawn, one at a time (f is there four times)
-    auto each_key = [&](auto f) {
-        constexpr int DEEP = 4;
-        const int from = max(0, piece0 * V - shift), to = min(n, piece1 * V - shift);
-        #pragma unroll 1
-        for(int i = from + lane; i < to; i += 32 * DEEP) {
-            float v[DEEP];
-            #pragma unroll
-            for(int d = 0; d < DEEP; d++) v[d] = i + d * 32 < to ? to_float(ld_plain(x + i + d * 32)) : __int_as_float(0xff800000);
-            #pragma unroll
-            for(int d = 0; d < DEEP; d++) {
-                const unsigned key = key_of(v[d]);
-                if(key != MASKED) f(key);
+    // f(logits) for the segment's classes, BATCH a thread at a time (-inf: none): their masses are worked out side by side, under the load of the next piece
+    constexpr int BATCH = 2;
+    auto each_batch = [&](auto f) {
+        union Piece { uint4 w; T e[V]; } u0, u1;
+        auto ask = [&](int p, Piece &u) {
+            const int i0 = p * V - shift;
+            if(p < piece1 && i0 >= 0 && i0 + V <= n) u.w = ld_plain(reinterpret_cast<const uint4 *>(x + i0));
+            else {
+                #pragma unroll
+                for(int e = 0; e < V; e++) u.e[e] = p < piece1 && i0 + e >= 0 && i0 + e < n ? ld_plain(x + i0 + e) : from_float<T>(__int_as_float(0xff800000));
             }
+        };
+        auto take = [&](const Piece &u) {
+            #pragma unroll
+            for(int e = 0; e < V; e += BATCH) {
+                float v[BATCH];
+                #pragma unroll
+                for(int d = 0; d < BATCH; d++) v[d] = to_float(u.e[e + d]);
+                f(v);
+            }
+        };
+        int p = piece0 + lane;
+        if(p >= piece1) return;
+        ask(p, u0);
+        #pragma unroll 1
+        for(;; p += 64) {
+            if(p + 32 < piece1) ask(p + 32, u1);
+            take(u0);
+            if(p + 32 >= piece1) break;
+            if(p + 64 < piece1) ask(p + 64, u0);
+            take(u1);
+            if(p + 64 >= piece1) break;
         }
     };
 
     // ---- the largest logit, its first place, and the groups' largest (a group: `parts` neighbouring threads)
-    if(tid < 64) sh.table[tid] = exp2(tid * (-1.0 / 64));
+    for(int i = tid; i < STEPS; i += THREADS) sh.table[i] = exp2(i * (-1.0 / STEPS));
     if(tid == 0) sh.cands = 0;
     float most = __int_as_float(0xff800000);
     int where = 0;
@@ -277,9 +316,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a)
         return;
     }
     Masses f;
-    f.top_key = top;
-    f.top = double(value_of(top));
+    f.top = value_of(top);
     f.factor = 1.4426950408889634074 / double(t);
+    f.top_t = double(f.top) * f.factor;
     f.one = double(1ull << a.bits);
     f.least = m > 0.0f ? fmin(double(m), 1.0) : 0.0;
     f.table = sh.table;
@@ -291,9 +330,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a)
     };
     auto point_in = [&](u64 whole) { return __umul64hi(uf > 0.0f ? (uf < 1.0f ? u64(double(uf) * 18446744073709551616.0) : ~0ull) : 0ull, whole); };
 
-    // Collects the classes with lo <= key <= hi (lo > MASKED): their number, and each thread's one of them, unsorted, if there are at most CAP.
-    // Two barriers, the second after the last look into another block's memory.
-    auto collect = [&](unsigned lo, unsigned hi, u64 &mine) {
+    // Collects the classes with lo <= key <= hi (lo > MASKED): their number, and in every block the list of them with their masses, in no order, if
+    // there are at most CAP.  The second barrier comes after the last look into another block's memory.
+    auto collect = [&](unsigned lo, unsigned hi) {
         const float low = value_of(lo), high = value_of(hi);
         each([&](float v, int i) {
             if(v >= low && v <= high) {
@@ -309,16 +348,44 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a)
             if(unsigned(tid) >= total && unsigned(tid) < total + c) { from = q; place = tid - total; }
             total += c;
         }
-        mine = 0;
+        u64 mine = 0;
         if(total <= CAP && unsigned(tid) < total) mine = parts > 1 ? peer(sh.cand + place, from) : sh.cand[place];
         everyone();
         if(tid == 0) sh.cands = 0;
-        return total;
+        if(mine) {
+            sh.list[tid] = mine;
+            sh.list_mass[tid] = f.mass(unsigned(mine >> 32));
+        }
+        __syncthreads();
+        return int(min(total, CAP + 1u));
     };
-    auto size_for = [](unsigned total) {
-        int size = 32;
-        while(size < int(total)) size <<= 1;
-        return size;
+    // threads to a class of a short list
+    auto share = [](int total) {
+        int e = 1;
+        while(e < 32 && total * e * 2 <= THREADS) e <<= 1;
+        return e;
+    };
+    // The list in order: a thread's class, its mass, its place, and the mass of what comes before it.  True for one thread of each class.
+    auto arrange = [&](int total, u64 &mine, u64 &mass, u64 &place, u64 &above) {
+        if(total <= COUNTED) {
+            const int e = share(total), me = tid / e;
+            const u64 id = me < total ? sh.list[me] : 0;
+            u64 p = 0, m = 0;
+            through(sh, total, e, [&](u64 c, u64 w) {
+                if(c > id) { p++; m += w; }
+            });
+            mine = id;
+            mass = me < total ? sh.list_mass[me] : 0;
+            place = sum_of(p, e);
+            above = sum_of(m, e);
+            return me < total && (tid & (e - 1)) == 0;
+        }
+        mine = sort(tid < total ? sh.list[tid] : 0, sh);
+        mass = tid < total ? f.mass(unsigned(mine >> 32)) : 0;
+        u64 all;
+        place = tid;
+        above = scan(mass, sh, flip, all) - mass;
+        return tid < total;
     };
 
     // ---- few classes are kept: all of them in one sorted list
@@ -326,11 +393,16 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a)
     if(few || n <= CAP) {
         unsigned floor_key = LOWEST;
         if(few) {
-            // the k-th largest of the groups' maxima, from the top bit down; done when exactly k of them are left (and but for the last eight bits:
-            // a little lower is as good)
-            unsigned at = 0;
+            // the k-th largest of the groups' maxima, from the top bit in which they differ down; done when exactly k of them are left (and but for the
+            // last eight bits: a little lower is as good)
+            const unsigned differ = __reduce_or_sync(0xffffffffu, group ^ top);
+            if(lane == 0) sh.group[warp] = differ;           // (the groups' maxima have been read)
+            __syncthreads();
+            const unsigned any = __reduce_or_sync(0xffffffffu, sh.group[lane & (WARPS - 1)]);
+            const int high = 31 - __clz(int(any | 1));
+            unsigned at = high == 31 ? 0 : top >> (high + 1) << (high + 1);
             #pragma unroll 1
-            for(int bit = 31; bit >= 8; bit--) {
+            for(int bit = high; bit >= 8; bit--) {
                 const unsigned higher = at | 1u << bit;
                 const int above = __syncthreads_count(group >= higher);
                 if(above >= k) at = higher;
@@ -338,57 +410,96 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a)
             }
             floor_key = max(at, LOWEST);
         }
-        u64 mine;
-        const unsigned total = collect(floor_key, top, mine);
+        const int total = collect(floor_key, top);
         if(total <= CAP) {
-            const int size = size_for(total);
-            if(part != 0 || tid >= size) return;
-            const u64 got = sort(mine, size, sh, size);
-            const unsigned key = unsigned(got >> 32);
-            const int kept_k = k > 0 && k < int(total) ? k : int(total);
-            const double w = tid < kept_k ? f.weight(key) : 0.0;
-            u64 mass = tid < kept_k ? f.whole(w) : 0, whole, run = scan(mass, sh, flip, whole, size);
-            if(p < 1.0f && run - mass >= share_of(whole)) mass = 0;
-            if(w < f.least) mass = 0;
-            // in index order: by ~index, the largest first, with the place of the mass
-            sh.all_mass[tid] = mass;
-            const u64 by_index = sort(mass ? (got & 0xffffffffull) << 32 | unsigned(tid) : 0, size, sh, size);
-            sync(size);
-            mass = by_index ? sh.all_mass[unsigned(by_index)] : 0;
-            run = scan(mass, sh, flip, whole, size);
-            const u64 target = point_in(whole);
-            if(mass && run > target && run - mass <= target) a.tokens[row] = int(~unsigned(by_index >> 32));
+            if(part != 0) return;
+            u64 mine, mass, place, above;
+            const bool one = arrange(total, mine, mass, place, above);
+            bool kept = one && !(k > 0 && place >= u64(k));
+            const u64 whole = sum_all(kept ? mass : 0, sh, flip);
+            if(p < 1.0f && place > 0 && above >= share_of(whole)) kept = false;
+            if(kept && f.least > 0.0 && f.weight(value_of(unsigned(mine >> 32))) < f.least) kept = false;
+            const u64 kept_mass = kept ? mass : 0, target = point_in(sum_all(kept_mass, sh, flip));
+            // and in index order: what has a larger ~index comes before
+            u64 before = 0, here = kept_mass, id = mine;
+            if(total <= COUNTED) {
+                const int e = share(total);
+                if(one) sh.list_mass[tid / e] = kept_mass;
+                __syncthreads();
+                through(sh, total, e, [&](u64 c, u64 w) {
+                    if(unsigned(c) > unsigned(mine)) before += w;
+                });
+                before = sum_of(before, e);
+            }
+            else {
+                sh.list_mass[tid] = kept_mass;
+                __syncthreads();
+                const u64 by_index = sort(kept_mass ? (mine & 0xffffffffull) << 32 | unsigned(tid) : 0, sh);
+                here = by_index ? sh.list_mass[unsigned(by_index)] : 0;
+                id = by_index >> 32;
+                u64 all;
+                before = scan(here, sh, flip, all) - here;
+            }
+            if(here && before <= target && before + here > target) a.tokens[row] = int(~unsigned(id));
             return;
         }
     }
 
     // ---- the ends of long prefixes
     const bool by_count = k > 0 && k < n, by_mass = p < 1.0f;
-    const float bin_scale = fminf(float(BINS) / (30.0f * t), 1e30f), top_value = value_of(top);
-    // bin of a key, 0 for the largest logits
-    auto bin_of = [&](unsigned key) { return key == top ? 0 : int(fminf((top_value - value_of(key)) * bin_scale, float(BINS - 1))); };
+    // Bins for the logits down to RANGE temperatures under the largest one; what is further down is summed up without one.
+    constexpr float RANGE = 20.0f;
+    const float bin_scale = fminf(float(BINS) / (RANGE * t), 1e30f), top_value = value_of(top);
+    // bin of a logit, 0 for the largest ones; BINS: none
+    auto bin_of = [&](float v) { return v == top_value ? 0 : int(fminf((top_value - v) * bin_scale, float(BINS))); };
     // Sums over bins of the classes with lo <= key <= hi, the same in every block; bits < 0: bins of logits, else of (hi - key) >> bits.  A mass is
-    // added in two 32-bit halves with a carry between them (64-bit additions in shared memory are loops).
+    // added in two 32-bit halves with a carry between them (64-bit additions in shared memory are loops).  rest_..: sums of what has no bin.
+    u64 rest_mass = 0, rest_count = 0;
     auto histogram = [&](unsigned lo, unsigned hi, int bits) {
         __syncthreads();
-        for(int i = tid; i < BINS; i += THREADS) sh.mass_lo[i] = sh.mass_hi[i] = sh.count[i] = 0;
+        for(int i = tid; i < BINS; i += THREADS) { sh.mass[i] = make_uint2(0, 0); sh.count[i] = 0; }
         __syncthreads();
-        each_key([&](unsigned key) {
-            if(key < lo || key > hi) return;
-            const int b = bits < 0 ? bin_of(key) : int((hi - key) >> bits);
-            const u64 mass = f.mass(key);
-            const unsigned low = unsigned(mass), was = atomicAdd(&sh.mass_lo[b], low), high = unsigned(mass >> 32) + (was + low < low);
-            if(high) atomicAdd(&sh.mass_hi[b], high);
-            atomicAdd(&sh.count[b], 1u);
+        u64 rest_m = 0, rest_c = 0;
+        const float low = value_of(lo), high = value_of(hi);
+        each_batch([&](const float (&v)[BATCH]) {
+            u64 mass[BATCH];
+            bool any = false;
+            #pragma unroll
+            for(int d = 0; d < BATCH; d++) any = any || (v[d] >= low && v[d] <= high);
+            if(!any) return;
+            #pragma unroll
+            for(int d = 0; d < BATCH; d++) mass[d] = f.mass(v[d]);
+            #pragma unroll
+            for(int d = 0; d < BATCH; d++) {
+                if(!(v[d] >= low && v[d] <= high)) continue;
+                const int b = bits < 0 ? bin_of(v[d]) : int((hi - key_of(v[d])) >> bits);
+                if(b >= BINS) {
+                    rest_m += mass[d];
+                    if(by_count) rest_c++;
+                    continue;
+                }
+                const unsigned low32 = unsigned(mass[d]), was = atomicAdd(&sh.mass[b].x, low32), high32 = unsigned(mass[d] >> 32) + (was + low32 < low32);
+                if(high32) atomicAdd(&sh.mass[b].y, high32);
+                if(by_count) atomicAdd(&sh.count[b], 1u);
+            }
         });
+        rest_m = sum_all(rest_m, sh, flip);
+        rest_c = sum_all(rest_c, sh, flip);
+        if(tid == 0) { sh.rest[0] = rest_m; sh.rest[1] = rest_c; }
         everyone();
+        rest_mass = rest_count = 0;
+        for(int q = 0; q < parts; q++) {
+            rest_mass += parts > 1 ? peer(sh.rest, q) : sh.rest[0];
+            rest_count += parts > 1 ? peer(sh.rest + 1, q) : sh.rest[1];
+        }
+        #pragma unroll 2
         for(int i = tid; i < BINS; i += THREADS) {
             u64 s = 0;
             unsigned c = 0;
             for(int q = 0; q < parts; q++) {
-                s += parts > 1 ? u64(peer(sh.mass_hi + i, q)) << 32 : u64(sh.mass_hi[i]) << 32;
-                s += parts > 1 ? peer(sh.mass_lo + i, q) : sh.mass_lo[i];
-                c += parts > 1 ? peer(sh.count + i, q) : sh.count[i];
+                const u64 *from = reinterpret_cast<const u64 *>(sh.mass + i);
+                s += parts > 1 ? peer(from, q) : *from;
+                if(by_count) c += parts > 1 ? peer(sh.count + i, q) : sh.count[i];
             }
             sh.all_mass[i] = s;
             sh.all_count[i] = c;
@@ -396,13 +507,18 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a)
         everyone();
     };
     constexpr int MINE = BINS / THREADS;
-    // The bin in which the running sum (of masses, or of numbers) reaches `want`: it, and the sums before it.
+    // The bin in which the running sum (of masses, or of numbers) reaches `want`: it, and the sums before it; BINS if that is in none.
     auto find_bin = [&](bool masses, u64 want, u64 &mass_before, u64 &count_before) {
-        u64 ms = 0, cs = 0, whole;
+        u64 ms = 0, cs = 0, all_m, all_c = 0;
         for(int i = 0; i < MINE; i++) { ms += sh.all_mass[MINE * tid + i]; cs += sh.all_count[MINE * tid + i]; }
         const u64 m_own = ms, c_own = cs;
-        ms = scan(ms, sh, flip, whole, THREADS) - m_own;
-        cs = scan(cs, sh, flip, whole, THREADS) - c_own;
+        ms = scan(ms, sh, flip, all_m) - m_own;
+        if(by_count) cs = scan(cs, sh, flip, all_c) - c_own;
+        if((masses ? all_m : all_c) < want) {
+            mass_before = all_m;
+            count_before = all_c;
+            return BINS;
+        }
         if((masses ? ms : cs) < want && (masses ? ms + m_own : cs + c_own) >= want) {
             int b = MINE * tid;
             for(;; b++) {                                    // (ends in one of the thread's bins, by the condition above)
@@ -420,63 +536,75 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a)
         count_before = sh.found[2];
         return int(sh.found[0]);
     };
-    // The end of the shortest prefix with `want` classes, or that much mass, and its mass.  The sums over the bins of all logits are in place.
+    // The end of the shortest prefix with `want` classes, or that much mass, and its mass.  The sums over the bins of logits are in place.
     auto find_cut = [&](bool masses, u64 want, u64 &mass) {
         constexpr int G = grain_bits<T>;
-        Cut c;
         u64 mass_before, count_before;
         int b = find_bin(masses, want, mass_before, count_before);
-        // the keys of that bin: from the least key with bin <= b up to the least one with bin < b
-        unsigned lo, hi = top;
-        {
-            unsigned l = LOWEST - 1, h = top;
+        // the keys of that bin (or of what has none): from the least key with bin <= b up to the least one with bin < b
+        // (a warp tries 32 keys at a time, least first: the bins fall as the keys rise)
+        auto least_key = [&](unsigned from, int most) {      // the least key >= from whose bin is <= most; top's is
+            unsigned l = from, size = top - from;            // it is in l .. l + size
             #pragma unroll 1
-            while(h - l > 1) { const unsigned mid = l + (h - l) / 2; if(bin_of(mid) <= b) h = mid; else l = mid; }
-            lo = h;
-            if(b > 0) {
-                l = lo - 1; h = top;
-                #pragma unroll 1
-                while(h - l > 1) { const unsigned mid = l + (h - l) / 2; if(bin_of(mid) < b) h = mid; else l = mid; }
-                hi = h - 1;
+            while(size > 0) {
+                const unsigned step = size / 32 + 1;
+                const unsigned reach = lane * (unsigned long long)step < size ? l + lane * step : top;
+                const unsigned yes = __ballot_sync(0xffffffffu, bin_of(value_of(reach)) <= most);
+                const int at = __ffs(yes) - 1;               // the first lane that has one (the last ones stand for top)
+                if(at == 0) return l;
+                if(at < 0) {
+                    l += 31 * step + 1;
+                    size = top - l;
+                    continue;
+                }
+                const unsigned end = min((unsigned long long)(at * (unsigned long long)step), (unsigned long long)size) + l;
+                l += (at - 1) * step + 1;
+                size = end - l;
             }
-        }
+            return l;
+        };
+        unsigned low = least_key(LOWEST, b);
+        unsigned hi = b > 0 ? least_key(low, b - 1) - 1 : top;
         mass = mass_before;
         u64 left = want - (masses ? mass_before : count_before);
-        unsigned equal = sh.all_count[b];
-        while(equal > CAP && lo >> G < hi >> G) {
+        bool many = b == BINS;                               // more classes than a list takes: divided further
+        Cut c;
+        for(;;) {
+            if(!many) {
+                const int total = collect(low, min(hi, top));
+                if(total <= CAP) {
+                    u64 mine, w, place, above;
+                    const bool one = arrange(total, mine, w, place, above);
+                    __syncthreads();                         // (found has been read)
+                    if(one && (masses ? above < left && above + w >= left : place + 1 == left)) {
+                        sh.found[0] = place;
+                        sh.found[1] = above + w;
+                        sh.found[2] = mine >> 32;
+                    }
+                    __syncthreads();
+                    c.key = unsigned(sh.found[2]);
+                    c.ties = __syncthreads_count(one && unsigned(mine >> 32) == c.key && place <= sh.found[0]);
+                    mass += sh.found[1];
+                    return c;
+                }
+                if(low >> G == hi >> G) break;
+            }
             int bits = G;
-            while((hi - lo) >> bits >= BINS) bits++;
+            while((hi - low) >> bits >= BINS) bits++;
             hi |= (1u << G) - 1;                             // (bins end between numbers)
-            histogram(lo, hi, bits);
+            histogram(low, hi, bits);
             b = find_bin(masses, left, mass_before, count_before);
             mass += mass_before;
             left -= masses ? mass_before : count_before;
-            equal = sh.all_count[b];
             hi -= unsigned(b) << bits;
-            lo = max(lo, hi - ((1u << bits) - 1));
+            low = max(low, hi - ((1u << bits) - 1));
+            many = false;
         }
-        if(equal > CAP) {                                    // more equal logits than are sorted at once
-            c.key = hi & 0x80000000u ? hi >> G << G : hi | ((1u << G) - 1);
-            const u64 w = f.mass(c.key), need = masses ? (left + w - 1) / w : left;
-            c.ties = unsigned(need);
-            mass += need * w;
-            return c;
-        }
-        u64 mine;
-        const unsigned total = collect(lo, min(hi, top), mine);
-        const u64 got = sort(mine, size_for(total), sh, THREADS);
-        const unsigned key = unsigned(got >> 32);
-        const bool in = unsigned(tid) < total;
-        u64 whole;
-        const u64 w = in ? f.mass(key) : 0, run = scan(w, sh, flip, whole, THREADS);
-        const bool last = in && (masses ? run >= left && run - w < left : u64(tid) + 1 == left);
-        __syncthreads();
-        if(last) { sh.found[0] = tid; sh.found[1] = run; sh.found[2] = key; }
-        __syncthreads();
-        const int at = int(sh.found[0]);
-        mass += sh.found[1];
-        c.key = unsigned(sh.found[2]);
-        c.ties = __syncthreads_count(in && tid <= at && key == c.key);
+        // more equal logits than a list takes
+        c.key = hi & 0x80000000u ? hi >> G << G : hi | ((1u << G) - 1);
+        const u64 w = f.mass(c.key), need = masses ? (left + w - 1) / w : left;
+        c.ties = unsigned(need);
+        mass += need * w;
         return c;
     };
 
@@ -485,8 +613,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a)
         histogram(LOWEST, top, -1);
         u64 whole = 0, number = 0;
         for(int i = 0; i < MINE; i++) { whole += sh.all_mass[MINE * tid + i]; number += sh.all_count[MINE * tid + i]; }
-        scan(whole, sh, flip, whole, THREADS);
-        scan(number, sh, flip, number, THREADS);
+        whole = sum_all(whole, sh, flip) + rest_mass;
+        number = by_count ? sum_all(number, sh, flip) + rest_count : 0;
         bool fresh = true;                                   // the sums are those of all logits
         if(by_count && u64(k) < number) {
             cut = find_cut(false, u64(k), whole);
@@ -503,11 +631,17 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a)
     {
         u64 sure = 0;
         unsigned ties = 0;
-        each_key([&](unsigned key) {
-            if(key == cut.key) ties++;
-            else if(key > cut.key) {
-                const double w = f.weight(key);
-                if(w >= f.least) sure += f.whole(w);
+        const float at = cut.key == MASKED ? __int_as_float(0xff800000) : value_of(cut.key);
+        each_batch([&](const float (&v)[BATCH]) {
+            bool any = false;
+            #pragma unroll
+            for(int d = 0; d < BATCH; d++) any = any || v[d] >= at;
+            if(!any) return;
+            #pragma unroll
+            for(int d = 0; d < BATCH; d++) {
+                const double w = f.weight(v[d]);
+                if(v[d] > at) sure += w >= f.least ? f.whole(w) : 0;
+                else if(v[d] == at && cut.key != MASKED) ties++;
             }
         });
         #pragma unroll
@@ -518,7 +652,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a)
     everyone();
     u64 tie_mass = 0;
     if(cut.key != MASKED) {
-        const double w = f.weight(cut.key);
+        const double w = f.weight(value_of(cut.key));
         if(w >= f.least) tie_mass = f.whole(w);
     }
     const int segs = parts * WARPS;
@@ -529,9 +663,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a)
     }
     everyone();
     u64 whole;
-    const u64 ties_before = scan(seg_ties, sh, flip, whole, THREADS) - seg_ties;
+    const u64 ties_before = scan(seg_ties, sh, flip, whole) - seg_ties;
     if(seg_ties && ties_before < cut.ties) seg += tie_mass * min(seg_ties, cut.ties - ties_before);
-    const u64 run = scan(seg, sh, flip, whole, THREADS), target = point_in(whole);
+    const u64 run = scan(seg, sh, flip, whole), target = point_in(whole);
     if(seg && run > target && run - seg <= target) { sh.found[0] = tid; sh.found[1] = run - seg; sh.found[2] = ties_before; }
     __syncthreads();
     const int seg_at = int(sh.found[0]);
@@ -546,14 +680,14 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a)
         const unsigned key = i < to ? key_of(to_float(ld_plain(x + i))) : MASKED;
         const bool tie = key != MASKED && key == cut.key;
         u64 all_ties = 0, all;
-        const u64 rank = cut.key != MASKED ? scan(tie ? 1 : 0, sh, flip, all_ties, THREADS) : 0;
+        const u64 rank = cut.key != MASKED ? scan(tie ? 1 : 0, sh, flip, all_ties) : 0;
         u64 mass = 0;
         if(tie) mass = ties_seen + rank <= cut.ties ? tie_mass : 0;
         else if(key > cut.key) {
-            const double w = f.weight(key);
+            const double w = f.weight(value_of(key));
             if(w >= f.least) mass = f.whole(w);
         }
-        const u64 to_here = before + scan(mass, sh, flip, all, THREADS);
+        const u64 to_here = before + scan(mass, sh, flip, all);
         if(mass && to_here > target && to_here - mass <= target) a.tokens[row] = i;
         before += all;
         ties_seen += all_ties;
@@ -565,9 +699,10 @@ template<typename T> dlp_status launch_sample(const SampleArgs &a, int rows, cud
 {
     const dlp_status st = allow_shared<sample_kernel<T>>(int(sizeof(Scratch)));
     if(st != DLP_OK) return st;
-    // blocks of a row: as many as there is room for (two on an SM), with 4096 classes or more to each
+    // Blocks of a row: as many as there is room for (two on an SM), with 4096 classes or more to each; and with many classes to a row two or more
+    // in any case: rows take very different times, and short blocks fill the gaps (256 rows of 150001 with settings of their own 321 -> 176 us).
     int parts = 1;
-    while(parts < MAX_PARTS && (long long)rows * parts <= sm_count() && a.classes / (parts * 2) >= 4096) parts *= 2;
+    while(parts < MAX_PARTS && (((long long)rows * parts <= sm_count() && a.classes / (parts * 2) >= 4096) || a.classes / (parts * 2) >= 32768)) parts *= 2;
     DLP_REQUIRE((long long)rows * parts < (1ll << 31), "too many rows");
     DLP_LAUNCH_PDL(launch_pdl_cluster(one_wave((long long)rows * parts, THREADS), parts, sample_kernel<T>, rows * parts, THREADS, sizeof(Scratch), stream, a),
                    "sample_kernel");
