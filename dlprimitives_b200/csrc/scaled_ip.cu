@@ -1,13 +1,15 @@
 // InnerProduct of 8-bit operands with a scale for each block of 128, on the sm_100a tensor cores:
 //     y[r][o] = act( sum_b xs[b][r] ws[o / 128][b] sum_{k in block b} x[r][k] w[o][k]  + bias[o] ).
 // The scales differ from block to block of K, so the tensor core sums one block (four tcgen05.mma of K = 32) into tensor memory and
-// the sum over blocks is kept in fp32 registers: warps read a block's 128 x BN products from tensor memory, multiply by the two scales
+// the sum over blocks is kept in fp32 registers: warps read a block's products from tensor memory, multiply by the two scales
 // and add, while the tensor core works on the next block in another part of tensor memory.  Both operands are K-major and come in
 // by tensor-map copies, 128 bytes (a block of K) wide, zero-filled beyond the matrices, so that no size needs padding.
-//   * rows of x are the tile's rows (many rows): a thread's products share one pair of scales;
-//   * rows of w are the tile's rows (few rows of x): a batch of 16 rows fills a tile's 16 columns instead of an eighth of its 128 rows.
-//     K is cut into parts over the blocks of a cluster, so that a product of few tiles reads its weights with the whole GPU; the parts are
-//     added through distributed shared memory in a fixed order.
+//
+// This file has the entry point, the choice of kernel, and the kernel for few rows; scaled_ip_pair.cu has the one for many.  With few rows the weights
+// are what is read, and a tile is 128 rows of w (the MMA's M) by 16 to 64 rows of x (its N): a batch of 16 rows fills a tile's 16 columns instead
+// of an eighth of its 128 rows.  K is cut into parts over the blocks of a cluster, so that a product of few tiles reads its weights with the whole GPU; the parts
+// are added through distributed shared memory in a fixed order.  Measured (captured, us; in brackets the bytes' time at a copy's 6.5 TB/s): one row 4096 -> 4096
+// 5.3 (2.6: launch, set-up and the cluster's sum are the rest), one row 4096 -> 24576 19.5 (15.4), 48 rows 23.6 (15.8), 64 rows 24.9 (16.0).
 // Every wait is bounded (device status word + abort flag).
 #include "scaled_ip.cuh"
 #include <algorithm>
@@ -348,9 +350,9 @@ template<int BN> static dlp_status launch_few(const Problem &p, cudaStream_t str
 }
 
 // Which kernel.  Up to 64 rows one tile of the few-rows kernel covers them all.  Beyond, it is measured time per block of K and round of tiles (us,
-// at full clocks): 0.64 for its 64-column tiles, two on an SM, which can be cut along K; 0.32 and 0.555 for pair tiles of 128 and 256 outputs, which
-// cannot, and have an end of 0.5 and 1.5 a round.  (Measured, 4096 inputs: 256 rows to 24576 outputs 67, 35, 42; 8192 inputs to 1000: 10.9, 26, 38;
-// 4096 rows to 24576: pair 435 and 407, and at 8192 rows 944 and 873, where the card's power limit holds both back.)
+// at full clocks): 0.64 for its 64-column tiles, two on an SM, which can be cut along K; 0.33 and 0.52 for pair tiles of 128 and 256 outputs, which
+// cannot, and have an end of 0.5 and 1.2 a round.  (Measured, each of the three, us: 128 rows, 4096 -> 24576 39.7, 34.5, 38.9; 256 rows, 8192 -> 1000 10.9,
+// 22.5, 33.5; 517 rows, 4096 -> 4096 23.5, 24.2, 21.5; 517 rows, 5000 -> 7100 61.8, 44.5, 47.8; 4096 rows, 4096 -> 24576 837, 447, 387.)
 static dlp_status dispatch(const Problem &p, cudaStream_t stream)
 {
     if(p.rows <= 16) return launch_few<16>(p, stream);
@@ -360,8 +362,8 @@ static dlp_status dispatch(const Problem &p, cudaStream_t stream)
     const int parts = few_parts(p, 64);
     const double few = rounds((long long)ceil_div(p.outputs, BM) * ceil_div(p.rows, 64) * parts, sm_count() * 2) * ceil_div(p.kblocks, parts) * 0.64;
     const long long row_tiles = ceil_div(p.rows, 2 * BM);
-    const double narrow = rounds(row_tiles * ceil_div(p.outputs, 128), sm_count() / 2) * (p.kblocks * 0.32 + 0.5);
-    const double wide = rounds(row_tiles * ceil_div(p.outputs, 256), sm_count() / 2) * (p.kblocks * 0.555 + 1.5);
+    const double narrow = rounds(row_tiles * ceil_div(p.outputs, 128), sm_count() / 2) * (p.kblocks * 0.33 + 0.5);
+    const double wide = rounds(row_tiles * ceil_div(p.outputs, 256), sm_count() / 2) * (p.kblocks * 0.52 + 1.2);
     if(few <= narrow && few <= wide) return launch_few<64>(p, stream);
     return launch_pair(p, narrow < wide ? 128 : 256, stream);
 }

@@ -1,9 +1,9 @@
 // InnerProduct of 8-bit operands with block scales, many rows: pairs of SMs share a tile of 256 rows x BN outputs (tcgen05 cta_group::2).
 //
-// A block of K (128) is four tcgen05.mma (M 256, N BN, K 32), into one of 512 / BN accumulators in tensor memory; the sum over blocks is
-// kept in fp32 registers, since the scales change from block to block:  acc += (xs[b][row] ws[o / 128][b]) * products.  That is a read of tensor
-// memory and an FMA for each product of a block, 128 x BN of them on each SM under the next block's MMAs: 256 cycles on the FMA pipes of the
-// 512 that the tensor core needs for N = 256.  Each SM holds half of the operands (128 rows of x, BN / 2 rows of w) in its shared memory: the
+// A block of K (128) is four tcgen05.mma (M 256, N 128, K 32) for each 128 outputs, into one of four accumulators in tensor memory; the sum over
+// blocks is kept in fp32 registers, since the scales change from block to block:  acc += (xs[b][row] ws[o / 128][b]) * products.  That is a read of
+// tensor memory and an FMA for each product of a block, 128 x BN of them on each SM under the next block's MMAs: 256 cycles on the FMA pipes of the
+// 512 that the tensor core needs for 256 outputs.  Each SM holds half of the operands (128 rows of x, BN / 2 rows of w) in its shared memory: the
 // pair reads a row of w once where two single SMs would read it twice.
 //   * one warp per SM issues the tensor-map copies of its half; both halves' bytes are counted on the leader's barrier;
 //   * one thread of the leader issues the MMAs of the pair; its commits go to both SMs;
@@ -11,6 +11,12 @@
 //   * two warps per SM bring in the scales, eight blocks of K at a time, and leave their products in shared memory.
 // Tiles are taken in turn (persistent blocks), eight row tiles at a time down the columns, so that what the SMs read at one time stays in L2.
 // Every wait is bounded.
+//
+// What bounds it: an accumulator goes round by MMA, commit to both SMs, the read of tensor memory, an arrival at the leader and the next issue, and four
+// of them do not hide all of that; on large products the card's power limit takes over.  8192 rows, 4096 -> 24576: 770 to 830 us (2.0 to
+// 2.1 PFLOP/s) in short series, 945 (1.75) in long ones at 990 W and 1.57 GHz.  What it came from, same product, us: 1736 with arrivals that released
+// the thread's other memory operations, too; 841 without, 804 with the scales through shared memory; 812 to 922 with accumulators of 256 columns, two
+// of them, measured in turn with this form.
 #define DLP_INLINE_WAITS
 #include "scaled_ip.cuh"
 #include <algorithm>
@@ -23,7 +29,7 @@ constexpr int WARP_COPY = 0, WARP_MMA = 1, WARP_SCALE0 = 2, WARP_SUM0 = 4;
 constexpr int NUM_THREADS = 384, SUM_WARPS = 8;
 constexpr int REGS_LAUNCH = 168, REGS_ISSUE = 56, REGS_SUM = 224;
 static_assert(REGS_ISSUE + 2 * REGS_SUM <= 3 * REGS_LAUNCH, "setmaxnreg draws on the launch's registers");
-constexpr int MAX_STAGES = 8, MAX_ACC = 4;
+constexpr int MAX_STAGES = 8, MAX_ACC = 4, N = 128;        // N: columns of an MMA, and of an accumulator
 constexpr int CHUNK = 8;                    // blocks of K whose scales are brought in together
 constexpr int SCALE_BYTES = CHUNK * 2 * BM * 4;             // [block][half of the columns][row]
 constexpr int STORE_BYTES = 2 * 4096;       // of a warp: two boxes of 32 rows of 128 bytes
@@ -83,7 +89,7 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
                       const Params q, int *status)
 {
     extern __shared__ unsigned char smem_raw[];
-    constexpr int ACC = 512 / BN;                            // accumulators in tensor memory
+    constexpr int H = BN / N, SETS = MAX_ACC / H;            // MMAs to a block of K; sets of as many accumulators in tensor memory
     constexpr int X_BYTES = BM * BK, W_BYTES = BN / 2 * BK, STAGE_BYTES = X_BYTES + W_BYTES;
     constexpr int COLS = BN / 2;                             // of a summing warp
     unsigned char *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -100,7 +106,7 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
 
     if(threadIdx.x == 0) {
         for(int s = 0; s < MAX_STAGES; s++) { mbar_init(&sh->full[s], 1); mbar_init(&sh->empty[s], 1); }
-        for(int a = 0; a < MAX_ACC; a++) { mbar_init(&sh->acc_full[a], 1); mbar_init(&sh->acc_empty[a], 2 * SUM_WARPS); }
+        for(int a = 0; a < MAX_ACC; a++) { mbar_init(&sh->acc_full[a], 1); mbar_init(&sh->acc_empty[a], 2 * SUM_WARPS / H); }
         for(int a = 0; a < 2; a++) { mbar_init(&sh->scale_full[a], 2); mbar_init(&sh->scale_empty[a], SUM_WARPS); }
         mbar_init(&sh->drain, 1);
         sh->abort_flag = 0;
@@ -127,14 +133,15 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
                 const uint32_t full0 = place_in(smem_u32(&sh->full[0]), 0), empty0 = smem_u32(&sh->empty[0]);
                 for(int t = first; t < tiles && live; t += step) {
                     const Tile w = tile_at(t, q);
-                    const int x_row = w.row * 2 * BM + int(rank) * BM, w_row = w.col * BN + int(rank) * (BN / 2);
+                    const int x_row = w.row * 2 * BM + int(rank) * BM, w_row = w.col * BN + int(rank) * (N / 2);
                     #pragma unroll 1
                     for(int kb = 0; kb < kblocks; kb++) {
                         if(!wait_quietly(empty0 + 8 * s, phase, abort_flag, status, SIP_EMPTY)) { live = false; break; }
                         const uint32_t slot = ring0 + s * STAGE_BYTES, bar = full0 + 8 * s;
                         if(rank == 0) mbar_arrive_expect_tx(&sh->full[s], 2 * STAGE_BYTES);
                         tma_load_pair(slot, &tm_x, kb * BK, x_row, bar);
-                        tma_load_pair(slot + X_BYTES, &tm_w, kb * BK, w_row, bar);
+                        #pragma unroll
+                        for(int h = 0; h < H; h++) tma_load_pair(slot + X_BYTES + h * (W_BYTES / H), &tm_w, kb * BK, w_row + h * N, bar);
                         count++;
                         if(++s == S) { s = 0; phase ^= 1; }
                     }
@@ -153,28 +160,33 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
         }
         else if(warp == WARP_MMA) {
             if(rank == 0 && elect_one()) {
-                constexpr uint32_t IDESC = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(2 * BM >> 4) << 24);     // fp32 sums of e4m3, K-major, M 256
+                constexpr uint32_t IDESC = (1u << 4) | (uint32_t(N >> 3) << 17) | (uint32_t(2 * BM >> 4) << 24);      // fp32 sums of e4m3, K-major, M 256
                 constexpr uint64_t DESC_HI = uint64_t((1024u >> 4) | (1u << 14) | (2u << 29)) << 32;   // 8-row groups 1024 bytes apart, version 1, SWIZZLE_128B
                 const uint32_t ring = ((ring0 & 0x3FFFF) >> 4) | (1u << 16);
                 const uint32_t full0 = smem_u32(&sh->full[0]), empty0 = smem_u32(&sh->empty[0]), acc_full0 = smem_u32(&sh->acc_full[0]), acc_empty0 = smem_u32(&sh->acc_empty[0]);
                 uint32_t s = 0, phase = 0, b = 0, b_phase = 1;
+                bool live = true;
                 const long long total = (long long)((tiles - first + step - 1) / step) * kblocks;
                 #pragma unroll 1
-                for(long long it = 0; it < total; it++) {
+                for(long long it = 0; it < total && live; it++) {
                     // (the operands have been there for a while; the accumulator is what is waited for)
                     if(!wait_quietly(full0 + 8 * s, phase, abort_flag, status, SIP_FULL)) break;
-                    const uint32_t xd = ring + s * (STAGE_BYTES >> 4), wd = xd + (X_BYTES >> 4), d = tmem_base + b * BN;
-                    if(!wait_quietly(acc_empty0 + 8 * b, b_phase, abort_flag, status, SIP_ACC_EMPTY)) break;
-                    tc_fence_after();
+                    const uint32_t xd = ring + s * (STAGE_BYTES >> 4);
                     #pragma unroll
-                    for(int j = 0; j < 4; j++)
-                        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                                     "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-                                     ::"r"(d), "l"(DESC_HI | (xd + 2 * j)), "l"(DESC_HI | (wd + 2 * j)), "r"(IDESC), "r"(j) : "memory");
-                    commit_pair(acc_full0 + 8 * b);
+                    for(int h = 0; h < H; h++) {
+                        const uint32_t wd = xd + ((X_BYTES + h * (W_BYTES / H)) >> 4), acc = b * H + h;
+                        if(!wait_quietly(acc_empty0 + 8 * acc, b_phase, abort_flag, status, SIP_ACC_EMPTY)) { live = false; break; }
+                        tc_fence_after();
+                        #pragma unroll
+                        for(int j = 0; j < 4; j++)
+                            asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                                         "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                                         ::"r"(tmem_base + acc * N), "l"(DESC_HI | (xd + 2 * j)), "l"(DESC_HI | (wd + 2 * j)), "r"(IDESC), "r"(j) : "memory");
+                        commit_pair(acc_full0 + 8 * acc);
+                    }
                     commit_pair(empty0 + 8 * s);
                     if(++s == S) { s = 0; phase ^= 1; }
-                    if(++b == ACC) { b = 0; b_phase ^= 1; }
+                    if(++b == SETS) { b = 0; b_phase ^= 1; }
                 }
             }
             __syncwarp();
@@ -226,7 +238,7 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SUM));
         const int me = warp - WARP_SUM0, quad = warp & 3, half = me >> 2;
         const uint32_t my_store = store0 + me * STORE_BYTES;
-        const uint32_t acc_empty0 = place_in(smem_u32(&sh->acc_empty[0]), 0), acc_full0 = smem_u32(&sh->acc_full[0]);
+        const uint32_t acc_empty0 = place_in(smem_u32(&sh->acc_empty[H == 1 ? 0 : half]), 0), acc_full0 = smem_u32(&sh->acc_full[H == 1 ? 0 : half]);
         const float2 clamp = act_clamp(q.act);
         const uint32_t my_scales = scales0 + (half * BM + quad * 32 + lane) * 4, scale_empty0 = smem_u32(&sh->scale_empty[0]), scale_full0 = smem_u32(&sh->scale_full[0]);
         const bool leader = lane == 0;
@@ -236,39 +248,51 @@ scaled_ip_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_con
             float acc[COLS];
             #pragma unroll
             for(int j = 0; j < COLS; j++) acc[j] = 0.0f;
-            #pragma unroll 1
-            for(int left = kblocks; left > 0; left -= CHUNK) {
-                slot ^= 1;
-                if(slot == 0) s_phase ^= 1;
-                warp_wait_quietly(scale_full0 + 8 * slot, s_phase, abort_flag, status, SIP_SCALE_FULL, leader);
-                if(*(volatile int *)abort_flag) break;
-                const int n = min(left, CHUNK);
-                uint32_t scale_at = my_scales + slot * SCALE_BYTES;
-                #pragma unroll 1
-                for(int i = 0; i < n; i++, it++, scale_at += 2 * BM * 4) {
-                    const uint32_t b = it % ACC;
-                    float s;
-                    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(s) : "r"(scale_at) : "memory");
-                    warp_wait_quietly(acc_full0 + 8 * b, (it / ACC) & 1, abort_flag, status, SIP_ACC_FULL, leader);
-                    tc_fence_after();
-                    const uint32_t taddr = tmem_base + (uint32_t(quad * 32) << 16) + b * BN + half * COLS;
-                    uint32_t v[2][32];
-                    tmem_ld(taddr, v[0]);
-                    #pragma unroll
-                    for(int g = 0; g < COLS / 32; g++) {
-                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                        if(g + 1 < COLS / 32) tmem_ld(taddr + (g + 1) * 32, v[(g + 1) & 1]);
-                        else {
-                            tc_fence_before();
-                            __syncwarp();
-                            arrive_at(leader, acc_empty0 + 8 * b);
-                        }
-                        #pragma unroll
-                        for(int j = 0; j < 32; j++) acc[g * 32 + j] = fmaf(__uint_as_float(v[g & 1][j]), s, acc[g * 32 + j]);
-                    }
+            // What a block of K costs beside its products -- waits, the trip to tensor memory -- runs under the last products of the block before:
+            // begin() makes the scale ready, waits for the accumulator and asks for its first 32 columns.
+            constexpr int G = COLS / 32;
+            static_assert(G % 2 == 0, "the two buffers are taken in turn");
+            uint32_t v[2][32];
+            float s, s_next = 0.0f;
+            uint32_t scale_at = 0, taddr = 0;
+            auto begin = [&](int kb) {
+                if(kb % CHUNK == 0) {
+                    slot ^= 1;
+                    if(slot == 0) s_phase ^= 1;
+                    warp_wait_quietly(scale_full0 + 8 * slot, s_phase, abort_flag, status, SIP_SCALE_FULL, leader);
+                    scale_at = my_scales + slot * SCALE_BYTES;
                 }
-                __syncwarp();
-                arrive_if(leader, scale_empty0 + 8 * slot);
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(s_next) : "r"(scale_at) : "memory");
+                scale_at += 2 * BM * 4;
+                const uint32_t b = it % SETS;
+                warp_wait_quietly(acc_full0 + 8 * b * H, (it / SETS) & 1, abort_flag, status, SIP_ACC_FULL, leader);
+                tc_fence_after();
+                taddr = tmem_base + (uint32_t(quad * 32) << 16) + b * BN + half * COLS;
+                tmem_ld(taddr, v[0]);
+            };
+            begin(0);
+            #pragma unroll 1
+            for(int kb = 0; kb < kblocks; kb++) {
+                s = s_next;
+                #pragma unroll
+                for(int g = 0; g < G; g++) {
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if(g + 1 < G) tmem_ld(taddr + (g + 1) * 32, v[(g + 1) & 1]);
+                    else {
+                        tc_fence_before();
+                        __syncwarp();
+                        arrive_at(leader, acc_empty0 + 8 * (it % SETS) * H);
+                        if(kb % CHUNK == CHUNK - 1 || kb + 1 == kblocks) arrive_if(leader, scale_empty0 + 8 * slot);
+                        it++;
+                        if(kb + 1 < kblocks) begin(kb + 1);
+                    }
+                    #pragma unroll
+                    for(int j = 0; j < 32; j++) acc[g * 32 + j] = fmaf(__uint_as_float(v[g & 1][j]), s, acc[g * 32 + j]);
+                }
+                if(kb % CHUNK == 0 && *(volatile int *)abort_flag) {
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    break;
+                }
             }
             live = live && !*(volatile int *)abort_flag;
             if(!live) break;
@@ -421,7 +445,7 @@ template<int BN> dlp_status launch_bn(const Problem &p, cudaStream_t stream)
     q.mapped = aligned_to(p.y, 16) && p.y_stride * size % 16 == 0 && p.y_stride * size < (1ull << 40);
     CUtensorMap mx, mw, my = {};
     st = encode_operand(mx, p.x, p.x_stride, p.rows, p.inputs, BM);
-    if(st == DLP_OK) st = encode_operand(mw, p.w, p.w_stride, p.outputs, p.inputs, BN / 2);
+    if(st == DLP_OK) st = encode_operand(mw, p.w, p.w_stride, p.outputs, p.inputs, N / 2);
     if(st == DLP_OK && q.mapped) st = encode_result(my, p);
     if(st != DLP_OK) return st;
     const int tiles = q.row_tiles * q.col_tiles, pairs = std::min(tiles, sm_count() / 2);
