@@ -1,8 +1,11 @@
 // Root-mean-square norm of rows, with the addition of a residual before it and an 8-bit form of the result:
 //     h = x + residual,   y = h / sqrt(mean(h^2) + eps) * weight.
 // A block of threads has a row in its registers between the sum of squares and the outputs, so that a row is read once (up to 32768 columns; longer
-// ones are read a second time, from L2).  What bounds it is memory: 8192 x 5120 bf16 with residual, 8-bit output: NORM_A.
-// Rows that start off 16-byte boundaries are read and written in aligned pieces all the same (block8.cuh): NORM_B.
+// ones are read a second time, from L2).  What bounds it is memory: 8192 x 5120 bf16 with residual and 8-bit output take 51 us, 5.8 TB/s of the
+// 6.5 that a copy reaches (82 us before a row stayed in registers and the next one's loads were under way, 60 before the arithmetic went two values to an
+// instruction); 8192 x 4096 fp32 without 40 us, 4.2 TB/s (45 with the weights kept, for which there are no registers).  Rows that start off 16-byte
+// boundaries are read and written in aligned pieces all the same (block8.cuh): 4000 x 5001 82 us (107 element by element), 1.7 TB/s: shifting words between
+// lanes takes instructions and registers, and 320 threads are all that an SM holds.  One row of 4096: 2.1 us, the launch.
 #include "block8.cuh"
 
 namespace dlp {
@@ -59,24 +62,26 @@ __device__ __forceinline__ void norm_out(const NormArgs &a, long long row, int c
     else store8<__nv_bfloat16, KIND>(static_cast<__nv_bfloat16 *>(a.y) + row * a.y_stride, c, a.cols, v);
 }
 
+// 64 registers to a thread, for two blocks of 512 to an SM, or 128.  (Rows off their boundaries with 80, for two blocks of 384: 4000 x 5001 takes the same
+// time, 30000 x 777 124 us for 90.)
 constexpr bool half_registers(int nv, int kind) { return nv <= 2 && kind == ROW_WHOLE; }
 
 // NV: pieces of eight columns that a thread keeps, a block's width apart, so that a warp has 256 consecutive columns, two blocks of the 8-bit form.
 // KIND: see Row8, of all tensors together.  A block takes rows in turn and asks for the next one as soon as the registers of this one's
 // words are free: the reduction, the arithmetic and the stores of a row run under the loads of the next.  The weights stay.
 template<typename T, int NV, int KIND>
-__global__ void __launch_bounds__(MAX_THREADS, half_registers(NV, KIND) ? 2 : 1) rms_norm_kernel(const NormArgs a, int rows)
+__global__ void __launch_bounds__(MAX_THREADS, half_registers(NV, KIND) ? 2 : 1) rms_norm_kernel(const NormArgs a, unsigned rows)
 {
     pdl_wait();
     __shared__ float part[2][MAX_THREADS / 32];
     typedef Row8<T, KIND> Row;
     const int cols = a.cols, stride = blockDim.x * 8, c0 = threadIdx.x * 8;
     const T *weight = static_cast<const T *>(a.weight);
-    const auto x_at = [&](long long row) { return static_cast<const T *>(a.x) + row * a.x_stride; };
-    const auto r_at = [&](long long row) { return static_cast<const T *>(a.residual) + row * a.residual_stride; };
-    constexpr bool KEEP_WEIGHT = NV * WORDS<T> <= 16;        // (as far as registers go)
+    const auto x_at = [&](unsigned row) { return static_cast<const T *>(a.x) + row * a.x_stride; };
+    const auto r_at = [&](unsigned row) { return static_cast<const T *>(a.residual) + row * a.residual_stride; };
+    constexpr bool KEEP_WEIGHT = NV * WORDS<T> <= (KIND == ROW_WHOLE && NV > 2 ? 16 : 8);      // (as far as registers go)
     Row xw[NV], rw[NV], ww[KEEP_WEIGHT ? NV : 1];
-    auto ask = [&](long long row) {
+    auto ask = [&](unsigned row) {
         #pragma unroll
         for(int i = 0; i < NV; i++) {
             xw[i].ask(x_at(row), c0 + i * stride, cols, x_at(0), static_cast<const T *>(a.x_end));
@@ -90,7 +95,7 @@ __global__ void __launch_bounds__(MAX_THREADS, half_registers(NV, KIND) ? 2 : 1)
     }
     int turn = 0;
     #pragma unroll 1
-    for(int row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
+    for(unsigned row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
         float h[NV][8];
         Pair squares = both(0.0f);
         #pragma unroll
@@ -108,7 +113,7 @@ __global__ void __launch_bounds__(MAX_THREADS, half_registers(NV, KIND) ? 2 : 1)
         float sum, odd;
         apart(squares, sum, odd);
         sum += odd;
-        if(row + int(gridDim.x) < rows) ask(row + int(gridDim.x));
+        if(row + gridDim.x < rows) ask(row + gridDim.x);
         const float f = inverse_root(block_sum(sum, part[turn]) / float(cols) + a.eps);
         #pragma unroll
         for(int i = 0; i < NV; i++) {
@@ -168,8 +173,8 @@ template<typename T, int NV>
 dlp_status launch_nv(const NormArgs &a, int rows, int threads, bool off, cudaStream_t stream)
 {
     const int blocks = std::min(rows, sm_count() * std::max(1, (half_registers(NV, off ? ROW_ANY : ROW_WHOLE) ? 1024 : 512) / threads));       // all of them resident
-    if(off) DLP_LAUNCH_PDL(launch_pdl(true, rms_norm_kernel<T, NV, ROW_ANY>, blocks, threads, 0, stream, a, rows), "rms_norm_kernel");
-    else DLP_LAUNCH_PDL(launch_pdl(true, rms_norm_kernel<T, NV, ROW_WHOLE>, blocks, threads, 0, stream, a, rows), "rms_norm_kernel");
+    if(off) DLP_LAUNCH_PDL(launch_pdl(true, rms_norm_kernel<T, NV, ROW_ANY>, blocks, threads, 0, stream, a, unsigned(rows)), "rms_norm_kernel");
+    else DLP_LAUNCH_PDL(launch_pdl(true, rms_norm_kernel<T, NV, ROW_WHOLE>, blocks, threads, 0, stream, a, unsigned(rows)), "rms_norm_kernel");
     return DLP_OK;
 }
 template<typename T>
