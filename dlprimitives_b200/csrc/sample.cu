@@ -17,6 +17,13 @@
 //   * Otherwise the end of a prefix is found from sums over 2048 bins of falling logits: the bin it lies in is collected, and divided
 //     further as long as it holds more than 512 classes.  Then the masses of the kept classes are summed by
 //     segments of the row, and the one segment that the random number points into is gone through.
+//
+// Measured (captured): one row of 32000 with k up to 300 16.3 us, 64 rows of 128000 bf16 without settings 32, with top-p 75, 256 rows of 150001 fp32 with
+// settings of their own 137.  Memory is not what bounds it (they are 128 KB, 16 MB and 154 MB): one row is a chain of barriers, short sorts and first
+// fetches of code, 8000 cycles to find the k-th largest, 5000 to collect, 13000 for the list; many rows are masses (about 30 instructions to a
+// class, 17000 cycles for 64000 on an SM) and sums over bins (two atomic additions to a class, 25000).  Tried: masses of fp32 pairs, within 2^-30, a tenth
+// less on rows without settings, nothing on the others; halves of the bins in arrays of their own, and barriers that a block only waits for when it
+// needs them: nothing.
 #include "block8.cuh"
 
 namespace dlp {
@@ -92,7 +99,7 @@ __device__ __forceinline__ unsigned peer(const unsigned *p, int rank)
 // 2^-r by the series of exp(-r ln 2), whose fourth term is under 2^-50.
 constexpr int STEPS = 1024;
 struct Masses {
-    double top_t, factor, one, least;            // factor: log2(e) / temperature; top_t: max times that; one: 2^bits; least: w of min-p
+    double top_t, factor, one;                   // factor: log2(e) / temperature; top_t: max times that; one: 2^bits
     float top;
     const double *table;                         // 2^(-j / STEPS)
     // No branches: a chain of dependent operations, of which several run side by side where several are asked for.
@@ -155,7 +162,7 @@ __device__ __forceinline__ u64 sum_all(u64 v, Scratch &sh, int &flip)
 }
 // Lists of up to CAP classes in shared memory.  Short ones are gone through, each class against each, by `each` neighbouring threads (a power of two, at
 // most 32) to a class that share the list: f(number, mass) for a thread's share.  Long ones are sorted.
-constexpr int COUNTED = 128;
+constexpr int COUNTED = 256;
 template<typename F> __device__ __forceinline__ void through(const Scratch &sh, int total, int each, F f)
 {
     #pragma unroll 4
@@ -273,6 +280,11 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a)
         }
     };
 
+    // (asked for early, all at once)
+    const float t = a.temperature ? ld_plain(a.temperature + row) : 1.0f, p = a.top_p ? ld_plain(a.top_p + row) : 1.0f;
+    const float m = a.min_p ? ld_plain(a.min_p + row) : 0.0f, uf = ld_plain(a.u + row);
+    const int asked = a.top_k ? ld_plain(a.top_k + row) : 0, k = t > 0.0f ? asked : 1;
+
     // ---- the largest logit, its first place, and the groups' largest (a group: `parts` neighbouring threads)
     for(int i = tid; i < STEPS; i += THREADS) sh.table[i] = exp2(i * (-1.0 / STEPS));
     if(tid == 0) sh.cands = 0;
@@ -291,10 +303,6 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a)
         best = other > best ? other : best;
     }
     if(lane == 0) sh.best[warp] = best;
-    const float t = a.temperature ? ld_plain(a.temperature + row) : 1.0f;
-    const bool greedy = !(t > 0.0f);
-    const int k = greedy ? 1 : (a.top_k ? ld_plain(a.top_k + row) : 0);
-    const float p = a.top_p ? ld_plain(a.top_p + row) : 1.0f, m = a.min_p ? ld_plain(a.min_p + row) : 0.0f, uf = ld_plain(a.u + row);
     everyone();
     {
         const int per_part = THREADS / parts;
@@ -320,8 +328,21 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a)
     f.factor = 1.4426950408889634074 / double(t);
     f.top_t = double(f.top) * f.factor;
     f.one = double(1ull << a.bits);
-    f.least = m > 0.0f ? fmin(double(m), 1.0) : 0.0;
     f.table = sh.table;
+    // min-p keeps the logits from `least_kept` on: the least one with exp((x - max) / t) >= m.  The estimate max + t ln m is right to a few units of
+    // fp32, and the lanes try the numbers around it.  (Classes under it need no mass: 64 rows of 128000 33 -> 29 us, where each mass was compared before.)
+    float least_kept = __int_as_float(0xff800000);
+    if(m >= 1.0f) least_kept = f.top;
+    else if(m > 0.0f && f.top < __int_as_float(0x7f800000)) {
+        const float guess = float(double(f.top) + double(t) * log(double(m)));
+        if(guess >= __int_as_float(0xff7fffff)) {            // (else all finite ones are kept)
+            const unsigned key = key_of(guess) + lane - 16;
+            const float x = value_of(key);
+            const bool in = key >= top || (key >= LOWEST && f.weight(x) >= double(m));
+            const unsigned yes = __ballot_sync(0xffffffffu, in);
+            least_kept = fminf(__shfl_sync(0xffffffffu, x, yes ? __ffs(yes) - 1 : 31), f.top);
+        }
+    }
     // the least whole number that is no less than p times `whole`
     auto share_of = [&](u64 whole) {
         const u64 pf = p > 0.0f ? u64(double(p) * 18446744073709551616.0) : 0;
@@ -396,9 +417,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a)
             // the k-th largest of the groups' maxima, from the top bit in which they differ down; done when exactly k of them are left (and but for the
             // last eight bits: a little lower is as good)
             const unsigned differ = __reduce_or_sync(0xffffffffu, group ^ top);
-            if(lane == 0) sh.group[warp] = differ;           // (the groups' maxima have been read)
+            if(lane == 0) sh.seg_ties[warp] = differ;        // (free yet; the groups' maxima may still be read by other blocks)
             __syncthreads();
-            const unsigned any = __reduce_or_sync(0xffffffffu, sh.group[lane & (WARPS - 1)]);
+            const unsigned any = __reduce_or_sync(0xffffffffu, sh.seg_ties[lane & (WARPS - 1)]);
             const int high = 31 - __clz(int(any | 1));
             unsigned at = high == 31 ? 0 : top >> (high + 1) << (high + 1);
             #pragma unroll 1
@@ -418,7 +439,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a)
             bool kept = one && !(k > 0 && place >= u64(k));
             const u64 whole = sum_all(kept ? mass : 0, sh, flip);
             if(p < 1.0f && place > 0 && above >= share_of(whole)) kept = false;
-            if(kept && f.least > 0.0 && f.weight(value_of(unsigned(mine >> 32))) < f.least) kept = false;
+            if(kept && value_of(unsigned(mine >> 32)) < least_kept) kept = false;
             const u64 kept_mass = kept ? mass : 0, target = point_in(sum_all(kept_mass, sh, flip));
             // and in index order: what has a larger ~index comes before
             u64 before = 0, here = kept_mass, id = mine;
@@ -631,16 +652,16 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a)
     {
         u64 sure = 0;
         unsigned ties = 0;
-        const float at = cut.key == MASKED ? __int_as_float(0xff800000) : value_of(cut.key);
+        const float at = cut.key == MASKED ? __int_as_float(0xff800000) : value_of(cut.key), least = fmaxf(at, least_kept);
         each_batch([&](const float (&v)[BATCH]) {
             bool any = false;
             #pragma unroll
-            for(int d = 0; d < BATCH; d++) any = any || v[d] >= at;
+            for(int d = 0; d < BATCH; d++) any = any || v[d] >= least;
             if(!any) return;
             #pragma unroll
             for(int d = 0; d < BATCH; d++) {
-                const double w = f.weight(v[d]);
-                if(v[d] > at) sure += w >= f.least ? f.whole(w) : 0;
+                const u64 mass = f.mass(v[d]);
+                if(v[d] > at) sure += v[d] >= least_kept ? mass : 0;
                 else if(v[d] == at && cut.key != MASKED) ties++;
             }
         });
@@ -651,10 +672,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a)
     }
     everyone();
     u64 tie_mass = 0;
-    if(cut.key != MASKED) {
-        const double w = f.weight(value_of(cut.key));
-        if(w >= f.least) tie_mass = f.whole(w);
-    }
+    if(cut.key != MASKED && value_of(cut.key) >= least_kept) tie_mass = f.mass(cut.key);
     const int segs = parts * WARPS;
     u64 seg = 0, seg_ties = 0;
     if(tid < segs) {
@@ -683,10 +701,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a)
         const u64 rank = cut.key != MASKED ? scan(tie ? 1 : 0, sh, flip, all_ties) : 0;
         u64 mass = 0;
         if(tie) mass = ties_seen + rank <= cut.ties ? tie_mass : 0;
-        else if(key > cut.key) {
-            const double w = f.weight(value_of(key));
-            if(w >= f.least) mass = f.whole(w);
-        }
+        else if(key > cut.key && value_of(key) >= least_kept) mass = f.mass(key);
         const u64 to_here = before + scan(mass, sh, flip, all);
         if(mass && to_here > target && to_here - mass <= target) a.tokens[row] = i;
         before += all;
@@ -700,7 +715,7 @@ template<typename T> dlp_status launch_sample(const SampleArgs &a, int rows, cud
     const dlp_status st = allow_shared<sample_kernel<T>>(int(sizeof(Scratch)));
     if(st != DLP_OK) return st;
     // Blocks of a row: as many as there is room for (two on an SM), with 4096 classes or more to each; and with many classes to a row two or more
-    // in any case: rows take very different times, and short blocks fill the gaps (256 rows of 150001 with settings of their own 321 -> 176 us).
+    // in any case: rows take very different times, and short blocks fill the gaps (256 rows of 150001 with settings of their own 321 -> 176 us when it came in).
     int parts = 1;
     while(parts < MAX_PARTS && (((long long)rows * parts <= sm_count() && a.classes / (parts * 2) >= 4096) || a.classes / (parts * 2) >= 32768)) parts *= 2;
     DLP_REQUIRE((long long)rows * parts < (1ll << 31), "too many rows");

@@ -154,6 +154,28 @@ def test_settings_at_their_ends():
         check(x, u, kw)
 
 
+@pytest.mark.parametrize("top,t,m", [(0.0, 1.0, 0.25), (3.3, 0.7, 0.05), (math.log(8.0), 1.0, 0.125), (-1000.5, 2.0, 0.9), (1e30, 1.0, 0.5),
+                                     (0.25, 1e-3, 1e-30), (2.0, 1e30, 0.5), (1.0, 1.0, 1.0), (0.0, 1.0, 1e-45)])
+@pytest.mark.parametrize("n", [40, 5003, 40000])
+def test_the_border_of_min_p(top, t, m, n):
+    # One class beside the largest, a few fp32 numbers around the border (these are 2^-24 of the border apart, an exponential in 64 bits is
+    # right to 2^-52), and far from it; u is near 1, so that the class drawn is the last one kept with a mass worth mentioning.
+    top, m = float(torch.tensor(top)), float(torch.tensor(m))
+    near = [torch.tensor(top + t * math.log(m), dtype=torch.float32).clamp(-3e38, top)]
+    for up in (math.inf, -math.inf):
+        v = near[0]
+        for _ in range(40):
+            v = torch.nextafter(v, torch.tensor(up))
+            near.append(v)
+    far = [top - 1e-6, top - 1.0, top - 50.0 * t, -3e38, 0.0, 1e-30, -1e-30]
+    second = torch.tensor([min(float(v), top) for v in near + far if math.isfinite(v)], dtype=torch.float32)
+    x = torch.full((len(second), n), -math.inf, device=DEV)
+    x[:, 0], x[:, n - 1] = top, second.to(DEV)
+    rows = len(second)
+    u = torch.full((rows,), 1 - 2.0 ** -24, device=DEV)
+    check(x, u, {"temperature": torch.full((rows,), t, device=DEV), "min_p": torch.full((rows,), m, device=DEV)})
+
+
 def test_rows_far_apart_and_off_boundaries():
     memory = torch.full((7 * 9001 + 5,), math.inf, device=DEV)
     for shift in (0, 1, 3):
