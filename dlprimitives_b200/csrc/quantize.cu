@@ -175,7 +175,7 @@ dlp_status dlp_quantize_fwd(const dlp_quantize_args *args, void *stream)
     DLP_REQUIRE(rows <= 1 || (x_stride >= (gate == DLP_GATE_NONE ? 1ll : 2ll) * cols && q_stride >= cols), "rows overlap");
     DLP_REQUIRE(block_rows == 1 ? cols <= SCALE_BLOCK || scale_stride >= rows : rows <= SCALE_BLOCK || scale_stride >= ceil_div(cols, SCALE_BLOCK),
                 "lines of scales overlap");
-    DLP_REQUIRE(block_rows == 1 || rows <= 65535 * SCALE_BLOCK, "too many rows");
+    DLP_REQUIRE(block_rows == 1 || rows <= (1 << 30), "too many rows");
     const size_t size = type_size(type);
     DLP_REQUIRE(aligned_to(x, size) && aligned_to(scales, 4), "a tensor is not aligned to its elements");
     const long long length = (rows - 1) * (rows > 1 ? x_stride : 0) + (gate == DLP_GATE_NONE ? 1ll : 2ll) * cols;

@@ -169,6 +169,21 @@ def test_quantize_weights(kind, rows, cols, extra, shift):
     assert torch.equal(memory.view(torch.uint8), guard.view(torch.uint8))
 
 
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantize_of_very_many_rows(block_rows):
+    # more blocks of 128 rows than a grid's second axis has; the last rows against the same rows by themselves
+    from dlprimitives_b200 import capi
+    rows, tail = 65536 * 128 + 130, 258
+    x = torch.randn(rows, 8, device=DEV).to(torch.bfloat16)
+    q, part = torch.empty(rows, 8, dtype=TYPES["e4m3"], device=DEV), torch.empty(tail, 8, dtype=TYPES["e4m3"], device=DEV)
+    scales = torch.empty((1, rows) if block_rows == 1 else (-(-rows // 128), 1), device=DEV)
+    part_scales = torch.empty((1, tail) if block_rows == 1 else (-(-tail // 128), 1), device=DEV)
+    capi.quantize(x, q, scales, block_rows=block_rows)
+    capi.quantize(x[-tail:], part, part_scales, block_rows=block_rows)
+    assert torch.equal(q[-tail:].view(torch.uint8), part.view(torch.uint8))
+    assert torch.equal(scales.flatten()[-part_scales.numel():], part_scales.flatten())
+
+
 def test_quantize_blocks_that_are_not_finite_or_zero():
     from dlprimitives_b200 import capi
     x = torch.randn(260, 384, device=DEV)
