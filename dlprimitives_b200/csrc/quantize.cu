@@ -1,14 +1,14 @@
 // The 8-bit form of a matrix, or of what a gated activation makes of a pair of matrices side by side: blocks of 128 columns of one row
-// (the left operand of an 8-bit product) or of 128 x 128 (its weights).  Memory bounds it where there is no gate (8192 x 8192: fp32 51 us, 6.6 TB/s; bf16
-// 39 us, 5.2 TB/s; weights 11000 x 4096 bf16 29 us, 4.7 TB/s); with one, the arithmetic does not quite go under it: 8192 x 12288 pairs 122 us, 4.2 TB/s,
-// of which memory alone would take 77.
+// (the left operand of an 8-bit product) or of 128 x 128 (its weights).  Memory bounds it where there is no gate (8192 x 8192: fp32 50 us, 6.8 TB/s; bf16
+// 39 us, 5.2 TB/s; weights 11000 x 4096 bf16 25 us, 5.4 TB/s); with one, the arithmetic does not quite go under it: 8192 x 12288 pairs 119 us, 4.3 TB/s,
+// of which memory alone would take 77.  Rows off 16-byte boundaries: 4000 x 5001 pairs 40 us, weights 11000 x 4097 41 us, 3.3 TB/s.
 #include "block8.cuh"
 
 namespace dlp {
 namespace {
 
 struct QuantArgs {
-    const void *x, *x_end;      // x_end: behind the last row
+    const void *x;
     unsigned char *q;
     float *scales;
     long long x_stride, q_stride, scale_stride;
@@ -38,7 +38,7 @@ __device__ __forceinline__ void gated2(float &a0, float &a1, float up0, float up
 
 constexpr int ROW_THREADS = 256, ROW_WARPS = ROW_THREADS / 32, ROW_PIECES = 2;
 
-// A warp takes ROW_PIECES pieces of 256 columns of a row, eight columns a lane of each; sixteen lanes hold a block.  All its loads are under way before the
+// A warp takes ROW_PIECES pieces of 256 columns of a row, two blocks, eight columns a lane of each.  All its loads are under way before the
 // first is used.  2^per_row_log2: warps of a block that share a row; blockIdx.y: blocks that do; KIND: see Row8.  (Blocks that stay, go from row to
 // row and have the next pieces' loads under way were slower, 139 against 121 us for 8192 x 12288 pairs: a block that ends makes room for one that
 // starts with its loads, which keeps memory busy under the others' arithmetic better than a fixed order within each warp.)
@@ -50,26 +50,24 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) quantize_rows_kernel(const Qua
     const long long row = (long long)blockIdx.x * (ROW_WARPS >> per_row_log2) + (warp >> per_row_log2);
     if(row >= a.rows) return;
     const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
-    const T *from = static_cast<const T *>(a.x), *to = static_cast<const T *>(a.x_end);
     unsigned char *q = a.q + row * a.q_stride;
     float *scale = a.scales + row;
     const int step = gridDim.y * per_row * (256 * ROW_PIECES);
     #pragma unroll 1
-    for(int c0 = (blockIdx.y * per_row + (warp & (per_row - 1))) * (256 * ROW_PIECES) + lane * 8; c0 - lane * 8 < cols; c0 += step) {
+    for(int c0 = (blockIdx.y * per_row + (warp & (per_row - 1))) * (256 * ROW_PIECES); c0 < cols; c0 += step) {
         Row8<T, KIND> w[ROW_PIECES], u[GATED ? ROW_PIECES : 1];
         #pragma unroll
         for(int i = 0; i < ROW_PIECES; i++) {
-            w[i].ask(x, c0 + i * 256, cols, from, to);
-            if(GATED) u[GATED ? i : 0].ask(x + cols, c0 + i * 256, cols, from, to);
+            w[i].ask(x, c0 + i * 256, lane, cols);
+            if(GATED) u[GATED ? i : 0].ask(x + cols, c0 + i * 256, lane, cols);
         }
         #pragma unroll
         for(int i = 0; i < ROW_PIECES; i++) {
-            const int c = c0 + i * 256;
             float v[8];
-            w[i].settle(x, c, cols, v);
+            w[i].settle(v);
             if(GATED) {
                 float up[8];
-                u[GATED ? i : 0].settle(x + cols, c, cols, up);
+                u[GATED ? i : 0].settle(up);
                 if(a.gate == DLP_GATE_SILU) {
                     #pragma unroll
                     for(int j = 0; j < 8; j += 2) gated2(v[j], v[j + 1], up[j], up[j + 1], DLP_GATE_SILU);
@@ -79,50 +77,89 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) quantize_rows_kernel(const Qua
                     for(int j = 0; j < 8; j += 2) gated2(v[j], v[j + 1], up[j], up[j + 1], DLP_GATE_GELU);
                 }
             }
-            const float s = block_scale(__reduce_max_sync(lane < 16 ? 0xffffu : 0xffff0000u, magnitude_bits(v)));
-            if((lane & 15) == 0 && c < cols) scale[(c / SCALE_BLOCK) * a.scale_stride] = s;
-            store_e4m3<KIND>(q, c, cols, pack_e4m3(v, s));
+            store_e4m3<KIND>(q, scale, a.scale_stride, c0 + i * 256, lane, cols, v);
         }
     }
 }
 
-// A block of 256 threads takes a block of 128 x 128 and keeps it in registers: sixteen lanes hold a row, a thread eight rows.
+// A block of threads takes a block of 128 x 128 and keeps it in registers, pairs of rows to a warp: sixteen lanes hold a row each in eight consecutive
+// columns of a lane (WHOLE), or all of them the one and then the other in every 32nd column (ANY: half as many pairs to a warp, since a load brings a
+// register one element).
+constexpr int block_threads(int kind) { return kind == ROW_WHOLE ? 256 : 512; }
 template<typename T, int KIND>
-__global__ void __launch_bounds__(256) quantize_blocks_kernel(const QuantArgs a, int across)
+__global__ void __launch_bounds__(block_threads(KIND), KIND == ROW_WHOLE ? 3 : 2) quantize_blocks_kernel(const QuantArgs a, int across)
 {
     pdl_wait();
-    __shared__ unsigned most[8];
+    constexpr int BLOCK_WARPS = block_threads(KIND) / 32, PAIRS = SCALE_BLOCK / 2 / BLOCK_WARPS;
+    __shared__ unsigned most[BLOCK_WARPS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int block_row = blockIdx.x / across, block_col = blockIdx.x - block_row * across;       // (a grid's second axis ends at 65535)
-    const int c = block_col * SCALE_BLOCK + (lane & 15) * 8, row0 = block_row * SCALE_BLOCK + warp * 2 + (lane >> 4);
-    Row8<T, KIND, 16> w[8];
-    const T *x[8];
-    const auto cols_of = [&](int i) { return row0 + i * 16 < a.rows ? a.cols : 0; };       // a row that is not there has no columns
-    #pragma unroll
-    for(int i = 0; i < 8; i++) {
-        x[i] = static_cast<const T *>(a.x) + (row0 + i * 16 < a.rows ? row0 + i * 16 : 0) * a.x_stride;
-        w[i].ask(x[i], c, cols_of(i), static_cast<const T *>(a.x), static_cast<const T *>(a.x_end));
+    const int row0 = block_row * SCALE_BLOCK + warp * PAIRS * 2 + (KIND == ROW_WHOLE ? lane >> 4 : 0);
+    const int col = block_col * SCALE_BLOCK + (KIND == ROW_WHOLE ? (lane & 15) * 8 : lane);
+    // element j of pair i, as far as it is another one's place: row and column after row0 and col
+    const auto row_of = [](int i, int j) { return 2 * i + (KIND == ROW_WHOLE ? 0 : j >> 2); };
+    const auto col_of = [](int j) { return KIND == ROW_WHOLE ? 0 : 32 * (j & 3); };
+    const auto there = [&](int i, int j) { return row0 + row_of(i, j) < a.rows && col + col_of(j) < a.cols; };
+    const bool full = (block_row + 1) * SCALE_BLOCK <= a.rows && (block_col + 1) * SCALE_BLOCK <= a.cols;
+    const T *x = static_cast<const T *>(a.x) + row0 * a.x_stride + col;
+    float v[PAIRS][8];
+    {
+        union { uint4 w[WORDS<T> / 4]; T e[8]; } u[PAIRS];
+        #pragma unroll
+        for(int i = 0; i < PAIRS; i++) {
+            if constexpr(KIND == ROW_WHOLE) {
+                #pragma unroll
+                for(int g = 0; g < WORDS<T> / 4; g++)
+                    u[i].w[g] = there(i, 0) ? ld_plain(reinterpret_cast<const uint4 *>(x + row_of(i, 0) * a.x_stride) + g) : make_uint4(0, 0, 0, 0);
+            }
+            else if(!full) {
+                #pragma unroll
+                for(int j = 0; j < 8; j++) u[i].e[j] = there(i, j) ? ld_plain(x + row_of(i, j) * a.x_stride + col_of(j)) : from_float<T>(0.0f);
+            }
+        }
+        if(KIND == ROW_ANY && full) {
+            #pragma unroll
+            for(int i = 0; i < PAIRS; i++)
+                #pragma unroll
+                for(int j = 0; j < 8; j++) u[i].e[j] = ld_plain(x + row_of(i, j) * a.x_stride + col_of(j));
+        }
+        #pragma unroll
+        for(int i = 0; i < PAIRS; i++)
+            #pragma unroll
+            for(int j = 0; j < 8; j++) v[i][j] = to_float(u[i].e[j]);
     }
-    float v[8][8];
     unsigned m = 0;
     #pragma unroll
-    for(int i = 0; i < 8; i++) {
-        w[i].settle(x[i], c, cols_of(i), v[i]);
-        m = max(m, magnitude_bits(v[i]));
-    }
+    for(int i = 0; i < PAIRS; i++) m = max(m, magnitude_bits(v[i]));
     m = __reduce_max_sync(0xffffffffu, m);
     if(lane == 0) most[warp] = m;
     __syncthreads();
     #pragma unroll
-    for(int i = 0; i < 8; i++) m = max(m, most[i]);
+    for(int i = 0; i < BLOCK_WARPS; i++) m = max(m, most[i]);
     const float s = block_scale(m);
+    const Quotient by(s);
     if(threadIdx.x == 0) a.scales[block_row * a.scale_stride + block_col] = s;
+    unsigned char *to = a.q + row0 * a.q_stride + col;
+    if(KIND == ROW_ANY && full) {
+        #pragma unroll
+        for(int i = 0; i < PAIRS; i++) {
+            const uint32_t q[2] = { by.pack(v[i], 0), by.pack(v[i], 4) };
+            #pragma unroll
+            for(int j = 0; j < 8; j++) to[row_of(i, j) * a.q_stride + col_of(j)] = (unsigned char)(q[j >> 2] >> (8 * (j & 3)));
+        }
+        return;
+    }
     #pragma unroll
-    for(int i = 0; i < 8; i++) {
-        const int row = row0 + i * 16;
-        const uint2 q = pack_e4m3(v[i], s);
-        unsigned char *to = a.q + (row < a.rows ? row : 0) * a.q_stride;
-        if(row < a.rows) store_e4m3<KIND>(to, c, a.cols, q);
+    for(int i = 0; i < PAIRS; i++) {
+        const uint32_t q[2] = { by.pack(v[i], 0), by.pack(v[i], 4) };
+        if constexpr(KIND == ROW_WHOLE) {
+            if(there(i, 0)) *reinterpret_cast<uint2 *>(to + row_of(i, 0) * a.q_stride) = make_uint2(q[0], q[1]);
+        }
+        else {
+            #pragma unroll
+            for(int j = 0; j < 8; j++)
+                if(there(i, j)) to[row_of(i, j) * a.q_stride + col_of(j)] = (unsigned char)(q[j >> 2] >> (8 * (j & 3)));
+        }
     }
 }
 
@@ -148,9 +185,9 @@ dlp_status launch_quantize(const QuantArgs &a, int block_rows, bool off, cudaStr
     const int across = ceil_div(a.cols, SCALE_BLOCK);
     const long long grid = (long long)across * ceil_div(a.rows, SCALE_BLOCK);
     DLP_REQUIRE(grid < 1ll << 31, "too large");
-    const bool early = one_wave(grid, 256);
-    if(off) DLP_LAUNCH_PDL(launch_pdl(early, quantize_blocks_kernel<T, ROW_ANY>, unsigned(grid), 256, 0, stream, a, across), "quantize_blocks_kernel");
-    else DLP_LAUNCH_PDL(launch_pdl(early, quantize_blocks_kernel<T, ROW_WHOLE>, unsigned(grid), 256, 0, stream, a, across), "quantize_blocks_kernel");
+    const bool early = one_wave(grid, block_threads(off ? ROW_ANY : ROW_WHOLE));
+    if(off) DLP_LAUNCH_PDL(launch_pdl(early, quantize_blocks_kernel<T, ROW_ANY>, unsigned(grid), block_threads(ROW_ANY), 0, stream, a, across), "quantize_blocks_kernel");
+    else DLP_LAUNCH_PDL(launch_pdl(early, quantize_blocks_kernel<T, ROW_WHOLE>, unsigned(grid), block_threads(ROW_WHOLE), 0, stream, a, across), "quantize_blocks_kernel");
     return DLP_OK;
 }
 
@@ -178,8 +215,7 @@ dlp_status dlp_quantize_fwd(const dlp_quantize_args *args, void *stream)
     DLP_REQUIRE(block_rows == 1 || rows <= (1 << 30), "too many rows");
     const size_t size = type_size(type);
     DLP_REQUIRE(aligned_to(x, size) && aligned_to(scales, 4), "a tensor is not aligned to its elements");
-    const long long length = (rows - 1) * (rows > 1 ? x_stride : 0) + (gate == DLP_GATE_NONE ? 1ll : 2ll) * cols;
-    const QuantArgs a = { x, static_cast<const char *>(x) + length * (long long)size, static_cast<unsigned char *>(q), scales, x_stride, q_stride, scale_stride, rows, cols, gate };
+    const QuantArgs a = { x, static_cast<unsigned char *>(q), scales, x_stride, q_stride, scale_stride, rows, cols, gate };
     // every row, and the second half of a pair's, on a 16-byte boundary (8 for the numbers) and a multiple of eight long?
     const bool off = !(cols % 8 == 0 && aligned_to(x, 16) && aligned_to(q, 8) && (rows == 1 || (x_stride * size % 16 == 0 && q_stride % 8 == 0)));
     if(type == DLP_TYPE_F32) return launch_quantize<float>(a, block_rows, off, (cudaStream_t)stream);

@@ -1,18 +1,18 @@
 // Root-mean-square norm of rows, with the addition of a residual before it and an 8-bit form of the result:
 //     h = x + residual,   y = h / sqrt(mean(h^2) + eps) * weight.
 // A block of threads has a row in its registers between the sum of squares and the outputs, so that a row is read once (up to 32768 columns; longer
-// ones are read a second time, from L2).  What bounds it is memory: 8192 x 5120 bf16 with residual and 8-bit output take 51 us, 5.8 TB/s of the
+// ones are read a second time, from L2).  What bounds it is memory: 8192 x 5120 bf16 with residual and 8-bit output take 52 us, 5.7 TB/s of the
 // 6.5 that a copy reaches (82 us before a row stayed in registers and the next one's loads were under way, 60 before the arithmetic went two values to an
-// instruction); 8192 x 4096 fp32 without 40 us, 4.2 TB/s (45 with the weights kept, for which there are no registers).  Rows that start off 16-byte
-// boundaries are read and written in aligned pieces all the same (block8.cuh): 4000 x 5001 82 us (107 element by element), 1.7 TB/s: shifting words between
-// lanes takes instructions and registers, and 320 threads are all that an SM holds.  One row of 4096: 2.1 us, the launch.
+// instruction); 8192 x 4096 fp32 without a residual 40 us, 4.2 TB/s (45 with the weights kept, for which there are no registers).  Rows off 16-byte
+// boundaries are read element by element, a warp's 32 at a time, and then it is the number of loads: 4000 x 5001 bf16 41 us, 3.5 TB/s, fp32 47, 6.0.
+// 1500 x 15001 62 us (68 in 512 threads).  One row of 4096: 2.3 us, the launch.
 #include "block8.cuh"
 
 namespace dlp {
 namespace {
 
 struct NormArgs {
-    const void *x, *residual, *weight, *x_end, *residual_end, *weight_end;       // .._end: behind the last row
+    const void *x, *residual, *weight;
     void *total, *y;
     float *scales;
     long long x_stride, residual_stride, total_stride, y_stride, scale_stride;
@@ -20,10 +20,12 @@ struct NormArgs {
     float eps;
 };
 
+// Threads of a block at most.  (ANY: see Row8.  Two pieces to a thread and its registers at 64 fill an SM with 1024 threads, in one block or more.)
 constexpr int MAX_THREADS = 512;
+constexpr int most_threads(int nv, int kind) { return kind == ROW_ANY && nv <= 2 ? 1024 : MAX_THREADS; }
 
 // Sum over the block; `part` is used in turn from call to call, so that one barrier a call is enough.
-__device__ __forceinline__ float block_sum(float v, float (&part)[MAX_THREADS / 32])
+template<int WARPS> __device__ __forceinline__ float block_sum(float v, float (&part)[WARPS])
 {
     const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     #pragma unroll
@@ -31,9 +33,9 @@ __device__ __forceinline__ float block_sum(float v, float (&part)[MAX_THREADS / 
     if(warps == 1) return v;
     if(lane == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = (lane & (MAX_THREADS / 32 - 1)) < warps ? part[lane & (MAX_THREADS / 32 - 1)] : 0.0f;
+    v = (lane & (WARPS - 1)) < warps ? part[lane & (WARPS - 1)] : 0.0f;
     #pragma unroll
-    for(int o = MAX_THREADS / 64; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    for(int o = WARPS / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 // 1 / sqrt(v), with a Newton step for the last bits of the approximation
@@ -43,55 +45,45 @@ __device__ __forceinline__ float inverse_root(float v)
     return v < __int_as_float(0x7f800000) ? fmaf(0.5f * f, fmaf(-v * f, f, 1.0f), f) : f;
 }
 
-// What becomes of eight values h of a row: total, and the output in its type.
+// What becomes of a lane's eight of 256 values h of a row: total, and the output in its type.
 template<typename T, int KIND>
-__device__ __forceinline__ void norm_out(const NormArgs &a, long long row, int c, float (&v)[8], const float (&g)[8], float f)
+__device__ __forceinline__ void norm_out(const NormArgs &a, long long row, int c0, int lane, float (&v)[8], const float (&g)[8], float f)
 {
-    const int lane = threadIdx.x & 31;
-    if(a.total) store8<T, KIND>(static_cast<T *>(a.total) + row * a.total_stride, c, a.cols, v);
+    if(a.total) store8<T, KIND>(static_cast<T *>(a.total) + row * a.total_stride, c0, lane, a.cols, v);
     #pragma unroll
     for(int j = 0; j < 8; j += 2) apart(pair(v[j], v[j + 1]) * both(f) * pair(g[j], g[j + 1]), v[j], v[j + 1]);
-    if(a.y_type == DLP_TYPE_E4M3) {
-        const float s = block_scale(__reduce_max_sync(lane < 16 ? 0xffffu : 0xffff0000u, magnitude_bits(v)));
-        unsigned char *y = static_cast<unsigned char *>(a.y) + row * a.y_stride;
-        if((lane & 15) == 0 && c < a.cols) a.scales[(c / SCALE_BLOCK) * a.scale_stride + row] = s;
-        store_e4m3<KIND>(y, c, a.cols, pack_e4m3(v, s));
-    }
-    else if(a.y_type == DLP_TYPE_F32) store8<float, KIND>(static_cast<float *>(a.y) + row * a.y_stride, c, a.cols, v);
-    else if(a.y_type == DLP_TYPE_F16) store8<__half, KIND>(static_cast<__half *>(a.y) + row * a.y_stride, c, a.cols, v);
-    else store8<__nv_bfloat16, KIND>(static_cast<__nv_bfloat16 *>(a.y) + row * a.y_stride, c, a.cols, v);
+    if(a.y_type == DLP_TYPE_E4M3) store_e4m3<KIND>(static_cast<unsigned char *>(a.y) + row * a.y_stride, a.scales + row, a.scale_stride, c0, lane, a.cols, v);
+    else if(a.y_type == DLP_TYPE_F32) store8<float, KIND>(static_cast<float *>(a.y) + row * a.y_stride, c0, lane, a.cols, v);
+    else if(a.y_type == DLP_TYPE_F16) store8<__half, KIND>(static_cast<__half *>(a.y) + row * a.y_stride, c0, lane, a.cols, v);
+    else store8<__nv_bfloat16, KIND>(static_cast<__nv_bfloat16 *>(a.y) + row * a.y_stride, c0, lane, a.cols, v);
 }
 
-// 64 registers to a thread, for two blocks of 512 to an SM, or 128.  (Rows off their boundaries with 80, for two blocks of 384: 4000 x 5001 takes the same
-// time, 30000 x 777 124 us for 90.)
-constexpr bool half_registers(int nv, int kind) { return nv <= 2 && kind == ROW_WHOLE; }
-
-// NV: pieces of eight columns that a thread keeps, a block's width apart, so that a warp has 256 consecutive columns, two blocks of the 8-bit form.
-// KIND: see Row8, of all tensors together.  A block takes rows in turn and asks for the next one as soon as the registers of this one's
-// words are free: the reduction, the arithmetic and the stores of a row run under the loads of the next.  The weights stay.
+// NV: pieces of 256 columns, two blocks of the 8-bit form, that a warp keeps, a block's width apart.  KIND: see Row8, of all tensors together.
+// WHOLE: a block takes rows in turn and asks for the next one as soon as the registers of this one's words are free: the reduction, the
+// arithmetic and the stores of a row run under the loads of the next; the weights stay as far as registers go.  ANY: a row to a block, so that more of them
+// fit an SM and run under one another.
 template<typename T, int NV, int KIND>
-__global__ void __launch_bounds__(MAX_THREADS, half_registers(NV, KIND) ? 2 : 1) rms_norm_kernel(const NormArgs a, unsigned rows)
+__global__ void __launch_bounds__(most_threads(NV, KIND), (NV <= 2 ? 1024 : MAX_THREADS) / most_threads(NV, KIND)) rms_norm_kernel(const NormArgs a, unsigned rows)
 {
     pdl_wait();
-    __shared__ float part[2][MAX_THREADS / 32];
+    __shared__ float part[2][most_threads(NV, KIND) / 32];
     typedef Row8<T, KIND> Row;
-    const int cols = a.cols, stride = blockDim.x * 8, c0 = threadIdx.x * 8;
+    const int cols = a.cols, lane = threadIdx.x & 31, stride = blockDim.x * 8, c0 = (threadIdx.x >> 5) * 256;
     const T *weight = static_cast<const T *>(a.weight);
-    const auto x_at = [&](unsigned row) { return static_cast<const T *>(a.x) + row * a.x_stride; };
-    const auto r_at = [&](unsigned row) { return static_cast<const T *>(a.residual) + row * a.residual_stride; };
-    constexpr bool KEEP_WEIGHT = NV * WORDS<T> <= (KIND == ROW_WHOLE && NV > 2 ? 16 : 8);      // (as far as registers go)
+    constexpr bool KEEP_WEIGHT = KIND == ROW_WHOLE ? NV * WORDS<T> <= (NV > 2 ? 16 : 8) : NV <= 2;
     Row xw[NV], rw[NV], ww[KEEP_WEIGHT ? NV : 1];
     auto ask = [&](unsigned row) {
+        const T *x = static_cast<const T *>(a.x) + row * a.x_stride, *r = static_cast<const T *>(a.residual) + row * a.residual_stride;
         #pragma unroll
         for(int i = 0; i < NV; i++) {
-            xw[i].ask(x_at(row), c0 + i * stride, cols, x_at(0), static_cast<const T *>(a.x_end));
-            if(a.residual) rw[i].ask(r_at(row), c0 + i * stride, cols, r_at(0), static_cast<const T *>(a.residual_end));
+            xw[i].ask(x, c0 + i * stride, lane, cols);
+            if(a.residual) rw[i].ask(r, c0 + i * stride, lane, cols);
         }
     };
     ask(blockIdx.x);
     if(KEEP_WEIGHT) {
         #pragma unroll
-        for(int i = 0; i < NV; i++) ww[KEEP_WEIGHT ? i : 0].ask(weight, c0 + i * stride, cols, weight, static_cast<const T *>(a.weight_end));
+        for(int i = 0; i < NV; i++) ww[KEEP_WEIGHT ? i : 0].ask(weight, c0 + i * stride, lane, cols);
     }
     int turn = 0;
     #pragma unroll 1
@@ -100,10 +92,10 @@ __global__ void __launch_bounds__(MAX_THREADS, half_registers(NV, KIND) ? 2 : 1)
         Pair squares = both(0.0f);
         #pragma unroll
         for(int i = 0; i < NV; i++) {
-            xw[i].settle(x_at(row), c0 + i * stride, cols, h[i]);
+            xw[i].settle(h[i]);
             if(a.residual) {
                 float b[8];
-                rw[i].settle(r_at(row), c0 + i * stride, cols, b);
+                rw[i].settle(b);
                 #pragma unroll
                 for(int j = 0; j < 8; j += 2) apart(pair(h[i][j], h[i][j + 1]) + pair(b[j], b[j + 1]), h[i][j], h[i][j + 1]);
             }
@@ -113,18 +105,18 @@ __global__ void __launch_bounds__(MAX_THREADS, half_registers(NV, KIND) ? 2 : 1)
         float sum, odd;
         apart(squares, sum, odd);
         sum += odd;
-        if(row + gridDim.x < rows) ask(row + gridDim.x);
+        if(KIND == ROW_WHOLE && row + gridDim.x < rows) ask(row + gridDim.x);
         const float f = inverse_root(block_sum(sum, part[turn]) / float(cols) + a.eps);
         #pragma unroll
         for(int i = 0; i < NV; i++) {
-            const int c = c0 + i * stride;
             Row w;
             if(KEEP_WEIGHT) w = ww[KEEP_WEIGHT ? i : 0];
-            else w.ask(weight, c, cols, weight, static_cast<const T *>(a.weight_end));
+            else w.ask(weight, c0 + i * stride, lane, cols);
             float g[8];
-            w.settle(weight, c, cols, g);
-            norm_out<T, KIND>(a, row, c, h[i], g, f);
+            w.settle(g);
+            norm_out<T, KIND>(a, row, c0 + i * stride, lane, h[i], g, f);
         }
+        if(KIND == ROW_ANY) return;
     }
 }
 
@@ -135,57 +127,61 @@ __global__ void __launch_bounds__(MAX_THREADS, 2) rms_norm_long_kernel(const Nor
     pdl_wait();
     __shared__ float part[MAX_THREADS / 32];
     const long long row = blockIdx.x;
-    const int cols = a.cols, stride = blockDim.x * 8;
+    const int cols = a.cols, lane = threadIdx.x & 31, stride = blockDim.x * 8, first = (threadIdx.x >> 5) * 256;
     const T *x = static_cast<const T *>(a.x) + row * a.x_stride, *weight = static_cast<const T *>(a.weight);
     const T *r = a.residual ? static_cast<const T *>(a.residual) + row * a.residual_stride : nullptr;
-    auto fetch = [&](int c, float (&h)[8]) {
+    auto fetch = [&](int c0, float (&h)[8]) {
         Row8<T, KIND> xw, rw;
-        xw.ask(x, c, cols, static_cast<const T *>(a.x), static_cast<const T *>(a.x_end));
-        if(r) rw.ask(r, c, cols, static_cast<const T *>(a.residual), static_cast<const T *>(a.residual_end));
-        xw.settle(x, c, cols, h);
+        xw.ask(x, c0, lane, cols);
+        if(r) rw.ask(r, c0, lane, cols);
+        xw.settle(h);
         if(r) {
             float b[8];
-            rw.settle(r, c, cols, b);
+            rw.settle(b);
             #pragma unroll
             for(int j = 0; j < 8; j++) h[j] += b[j];
         }
     };
     float sum = 0.0f;
-    for(int c0 = 0; c0 < cols; c0 += stride) {
+    for(int c0 = first; c0 < cols; c0 += stride) {
         float h[8];
-        fetch(c0 + threadIdx.x * 8, h);
+        fetch(c0, h);
         #pragma unroll
         for(int j = 0; j < 8; j++) sum += h[j] * h[j];
     }
     const float f = inverse_root(block_sum(sum, part) / float(cols) + a.eps);
-    for(int c0 = 0; c0 < cols; c0 += stride) {
-        const int c = c0 + threadIdx.x * 8;
+    for(int c0 = first; c0 < cols; c0 += stride) {
         float h[8], g[8];
         Row8<T, KIND> w;
-        w.ask(weight, c, cols, weight, static_cast<const T *>(a.weight_end));
-        fetch(c, h);
-        w.settle(weight, c, cols, g);
-        norm_out<T, KIND>(a, row, c, h, g, f);
+        w.ask(weight, c0, lane, cols);
+        fetch(c0, h);
+        w.settle(g);
+        norm_out<T, KIND>(a, row, c0, lane, h, g, f);
     }
 }
 
 template<typename T, int NV>
 dlp_status launch_nv(const NormArgs &a, int rows, int threads, bool off, cudaStream_t stream)
 {
-    const int blocks = std::min(rows, sm_count() * std::max(1, (half_registers(NV, off ? ROW_ANY : ROW_WHOLE) ? 1024 : 512) / threads));       // all of them resident
-    if(off) DLP_LAUNCH_PDL(launch_pdl(true, rms_norm_kernel<T, NV, ROW_ANY>, blocks, threads, 0, stream, a, unsigned(rows)), "rms_norm_kernel");
-    else DLP_LAUNCH_PDL(launch_pdl(true, rms_norm_kernel<T, NV, ROW_WHOLE>, blocks, threads, 0, stream, a, unsigned(rows)), "rms_norm_kernel");
+    const int resident = std::min(rows, sm_count() * std::max(1, (NV <= 2 ? 2 : 1) * MAX_THREADS / threads));
+    if constexpr(NV != 4) {                                  // (what is ANY has two pieces in 1024 threads where four would be in 512)
+        if(off) {
+            DLP_LAUNCH_PDL(launch_pdl(one_wave(rows, threads), rms_norm_kernel<T, NV, ROW_ANY>, rows, threads, 0, stream, a, unsigned(rows)), "rms_norm_kernel");
+            return DLP_OK;
+        }
+    }
+    DLP_LAUNCH_PDL(launch_pdl(true, rms_norm_kernel<T, NV, ROW_WHOLE>, resident, threads, 0, stream, a, unsigned(rows)), "rms_norm_kernel");
     return DLP_OK;
 }
 template<typename T>
 dlp_status launch_norm(const NormArgs &a, int rows, bool off, cudaStream_t stream)
 {
-    // With few rows each has as many threads as it can use (latency); with many, threads that keep two pieces or more have more loads under way.
-    const int pieces = ceil_div(a.cols, 8), least = rows <= 2 * sm_count() ? 1 : 2;
+    // With few rows each has as many warps as it can use (latency); with many, warps that keep two pieces or more have more loads under way.
+    const int pieces = ceil_div(a.cols, 256), least = rows <= 2 * sm_count() ? 1 : 2;
     int nv = 1;
-    while(nv < 8 && (nv < least || ceil_div(pieces, nv) > MAX_THREADS)) nv *= 2;
-    const int threads = round_up(ceil_div(pieces, nv), 32);
-    if(threads > MAX_THREADS) {
+    while(nv < 8 && (nv < least || ceil_div(pieces, nv) > most_threads(nv, off ? ROW_ANY : ROW_WHOLE) / 32)) nv *= 2;
+    const int threads = ceil_div(pieces, nv) * 32;
+    if(threads > most_threads(nv, off ? ROW_ANY : ROW_WHOLE)) {
         const bool early = one_wave(rows, MAX_THREADS);
         if(off) DLP_LAUNCH_PDL(launch_pdl(early, rms_norm_long_kernel<T, ROW_ANY>, rows, MAX_THREADS, 0, stream, a), "rms_norm_long_kernel");
         else DLP_LAUNCH_PDL(launch_pdl(early, rms_norm_long_kernel<T, ROW_WHOLE>, rows, MAX_THREADS, 0, stream, a), "rms_norm_long_kernel");
@@ -224,10 +220,7 @@ dlp_status dlp_rms_norm_fwd(const dlp_rms_norm_args *args, void *stream)
     const size_t size = type_size(type), y_size = type_size(y_type);
     DLP_REQUIRE(aligned_to(x, size) && aligned_to(weight, size) && aligned_to(y, y_size) && (!residual || aligned_to(residual, size)) &&
                 (!total || aligned_to(total, size)) && (!scales || aligned_to(scales, 4)), "a tensor is not aligned to its elements");
-    const auto end = [rows = args->rows, cols = args->cols](const void *p, long long stride, size_t element) -> const void * {
-        return p ? static_cast<const char *>(p) + ((rows - 1) * (rows > 1 ? stride : 0) + cols) * (long long)element : nullptr;
-    };
-    NormArgs a = { x, residual, weight, end(x, x_stride, size), end(residual, residual_stride, size), end(weight, 0, size), total, y, scales, x_stride, residual_stride, total_stride, y_stride, scale_stride, cols, y_type, eps };
+    NormArgs a = { x, residual, weight, total, y, scales, x_stride, residual_stride, total_stride, y_stride, scale_stride, cols, y_type, eps };
     const auto rows_on = [rows = args->rows](const void *p, long long stride, size_t element, size_t n) { return aligned_to(p, n) && (rows == 1 || stride * element % n == 0); };
     const bool off = !(cols % 8 == 0 && rows_on(x, x_stride, size, 16) && aligned_to(weight, 16) && (!residual || rows_on(residual, residual_stride, size, 16)) &&
                        (!total || rows_on(total, total_stride, size, 16)) && rows_on(y, y_stride, y_size, y_type == DLP_TYPE_E4M3 ? 8 : 16));
