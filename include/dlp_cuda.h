@@ -272,8 +272,8 @@ DLP_API dlp_status dlp_batchnorm_inference_fwd(const float *x, float *y, int bat
  * beside InnerProduct, BatchNorm, Activation and Softmax above).  Forward only.
  *
  * Matrices are row-major with unit stride along a row; strides are in elements and may be anything that keeps rows apart.  Tensors of a
- * call may not overlap, unless its comment says so.  Elements past a row's end (padding up to its stride) are not written, and what they
- * hold has no effect; rows past the last one are neither read nor written.
+ * call may not overlap, unless its comment says so.  Elements past a row's end (padding up to its stride) and rows past the last one
+ * are neither read nor written.
  *
  * The 8-bit form of a matrix: e4m3 numbers and an fp32 scale for each block, value = number * scale, with
  * scale = max(largest magnitude / 448, 2^-126) and number = value / scale rounded to the nearest (ties to even).  A block with a NaN or
