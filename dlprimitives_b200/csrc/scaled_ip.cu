@@ -317,12 +317,14 @@ dlp_status encode_result(CUtensorMap &map, const Problem &p)
     return encode_2d(map, type, p.y, p.outputs, p.rows, p.y_stride * size, 128 / size, 32);
 }
 
-// Parts of K that fill the places on the SMs.
+// Parts of K that give every SM a block; and a second one where parts stay ten blocks of K long (us, parts: 8 rows, 2000 -> 12000 7.8 one, 9.4 two; 32 rows,
+// 5000 -> 7100 15.0 two, 12.9 four; one row, 4096 -> 4096 8.2 one, 6.5 two, 5.5 four, 5.5 eight).  Parts that start a second round do not pay (48 rows,
+// 4096 -> 24576 24 one, 35 two, 36 three).
 static int few_parts(const Problem &p, int bn)
 {
-    const long long tiles = (long long)ceil_div(p.outputs, BM) * ceil_div(p.rows, bn), slots = sm_count() * 2;
+    const long long tiles = (long long)ceil_div(p.outputs, BM) * ceil_div(p.rows, bn), sms = sm_count();
     int parts = 1;
-    while(parts < MAX_CLUSTER && parts * 2 <= p.kblocks && tiles * parts * 2 <= slots) parts *= 2;
+    while(parts < MAX_CLUSTER && tiles * parts * 2 <= (p.kblocks >= parts * 2 * 10 ? 2 * sms : sms) && parts * 2 <= p.kblocks) parts *= 2;
     return parts;
 }
 
