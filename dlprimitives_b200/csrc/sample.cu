@@ -20,7 +20,7 @@
 //
 // Measured (captured): one row of 32000 with k up to 300 16.3 us, 64 rows of 128000 bf16 without settings 32, with top-p 75, 256 rows of 150001 fp32 with
 // settings of their own 137.  Memory is not what bounds it (they are 128 KB, 16 MB and 154 MB): one row is a chain of barriers, short sorts and first
-// fetches of code, 8000 cycles to find the k-th largest, 5000 to collect, 13000 for the list; many rows are masses (about 30 instructions to a
+// fetches of code, 7500 cycles up to the k-th largest, 5500 to collect, 13000 for the list; many rows are masses (about 30 instructions to a
 // class, 17000 cycles for 64000 on an SM) and sums over bins (two atomic additions to a class, 25000).  Tried: masses of fp32 pairs, within 2^-30, a tenth
 // less on rows without settings, nothing on the others; halves of the bins in arrays of their own, and barriers that a block only waits for when it
 // needs them: nothing.

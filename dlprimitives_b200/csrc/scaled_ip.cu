@@ -9,7 +9,7 @@
 // are what is read, and a tile is 128 rows of w (the MMA's M) by 16 to 64 rows of x (its N): a batch of 16 rows fills a tile's 16 columns instead
 // of an eighth of its 128 rows.  K is cut into parts over the blocks of a cluster, so that a product of few tiles reads its weights with the whole GPU; the parts
 // are added through distributed shared memory in a fixed order.  Measured (captured, us; in brackets the bytes' time at a copy's 6.5 TB/s): one row 4096 -> 4096
-// 5.3 (2.6: launch, set-up and the cluster's sum are the rest), one row 4096 -> 24576 19.5 (15.4), 48 rows 23.6 (15.8), 64 rows 24.9 (16.0).
+// 5.1 (2.6: launch, set-up and the cluster's sum are the rest), one row 4096 -> 24576 19.2 (15.4), 48 rows 23.4 (15.8), 64 rows 24.7 (16.0).
 // Every wait is bounded (device status word + abort flag).
 #include "scaled_ip.cuh"
 #include <algorithm>
