@@ -130,7 +130,7 @@ __device__ __forceinline__ float block_scale(unsigned magnitude)
 {
     const float m = __uint_as_float(magnitude);
     const float s0 = m * (1.0f / 448.0f), s = fmaf(fmaf(-448.0f, s0, m), 1.0f / 448.0f, s0);
-    return m < 5.2656e-36f ? 1.17549435e-38f : (magnitude < 0x7f800000u ? s : m);          // 448 * 2^-126 (under it 2^-126); infinite and NaN stay
+    return m < 0x1.cp-118f ? 0x1p-126f : (magnitude < 0x7f800000u ? s : m);                // under 448 * 2^-126: 2^-126; infinite and NaN stay
 }
 // Four numbers of the block, the first in the lowest byte: v / s, by a product with the approximate 1 / s and a correction of its remainder (a Newton step
 // of the quotient, after which it is the rounded one but for rare last units), then to the nearest e4m3, ties to even.
