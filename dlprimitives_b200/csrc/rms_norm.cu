@@ -45,6 +45,31 @@ __device__ __forceinline__ float inverse_root(float v)
     return v < __int_as_float(0x7f800000) ? fmaf(0.5f * f, fmaf(-v * f, f, 1.0f), f) : f;
 }
 
+// Where finite values have a sum of squares beyond fp32 (their rms is over 2^64 / sqrt(cols) then), 1 / sqrt(mean(h^2) + eps) comes out as 0.  The row is read again
+// then for the sum of (2^-96 h)^2, which is neither beyond fp32 nor lost; an infinity among the values makes that one infinite, too, and the result 0 again.
+// The sum is the same in every thread of the block, so all of them come here together, and nobody has written a total yet.
+// (Out of line and element by element, so that it takes no registers from the path without: the same from the row in registers cost bf16 rows of 20480 with
+// residual 85 -> 100 us.)
+template<typename T, int WARPS> __device__ __noinline__ float inverse_of_large(const T *x, const T *r, int cols, float eps, float (&part)[WARPS])
+{
+    constexpr float S = 0x1p-96f;
+    float again = 0.0f;
+    #pragma unroll 1
+    for(int c = threadIdx.x; c < cols; c += blockDim.x) {
+        const float h = (to_float(ld_plain(x + c)) + (r ? to_float(ld_plain(r + c)) : 0.0f)) * S;
+        again = fmaf(h, h, again);
+    }
+    return inverse_root(block_sum(again, part) / float(cols) + eps * S * S) * S;
+}
+template<typename T, int WARPS> __device__ __forceinline__ float inverse_rms(float sum, const NormArgs &a, long long row, float (&part)[WARPS])
+{
+    float f = inverse_root(sum / float(a.cols) + a.eps);
+    if(f == 0.0f)
+        f = inverse_of_large(static_cast<const T *>(a.x) + row * a.x_stride, a.residual ? static_cast<const T *>(a.residual) + row * a.residual_stride : nullptr,
+                             a.cols, a.eps, part);
+    return f;
+}
+
 // What becomes of a lane's eight of 256 values h of a row: total, and the output in its type.
 template<typename T, int KIND>
 __device__ __forceinline__ void norm_out(const NormArgs &a, long long row, int c0, int lane, float (&v)[8], const float (&g)[8], float f)
@@ -66,7 +91,7 @@ template<typename T, int NV, int KIND>
 __global__ void __launch_bounds__(most_threads(NV, KIND), (NV <= 2 ? 1024 : MAX_THREADS) / most_threads(NV, KIND)) rms_norm_kernel(const NormArgs a, unsigned rows)
 {
     pdl_wait();
-    __shared__ float part[2][most_threads(NV, KIND) / 32];
+    __shared__ float part[3][most_threads(NV, KIND) / 32];           // in turn from row to row, and for a second sum
     typedef Row8<T, KIND> Row;
     const int cols = a.cols, lane = threadIdx.x & 31, stride = blockDim.x * 8, c0 = (threadIdx.x >> 5) * 256;
     const T *weight = static_cast<const T *>(a.weight);
@@ -106,7 +131,7 @@ __global__ void __launch_bounds__(most_threads(NV, KIND), (NV <= 2 ? 1024 : MAX_
         apart(squares, sum, odd);
         sum += odd;
         if(KIND == ROW_WHOLE && row + gridDim.x < rows) ask(row + gridDim.x);
-        const float f = inverse_root(block_sum(sum, part[turn]) / float(cols) + a.eps);
+        const float f = inverse_rms<T>(block_sum(sum, part[turn]), a, row, part[2]);
         #pragma unroll
         for(int i = 0; i < NV; i++) {
             Row w;
@@ -125,7 +150,7 @@ template<typename T, int KIND>
 __global__ void __launch_bounds__(MAX_THREADS, 2) rms_norm_long_kernel(const NormArgs a)
 {
     pdl_wait();
-    __shared__ float part[MAX_THREADS / 32];
+    __shared__ float part[2][MAX_THREADS / 32];
     const long long row = blockIdx.x;
     const int cols = a.cols, lane = threadIdx.x & 31, stride = blockDim.x * 8, first = (threadIdx.x >> 5) * 256;
     const T *x = static_cast<const T *>(a.x) + row * a.x_stride, *weight = static_cast<const T *>(a.weight);
@@ -149,7 +174,7 @@ __global__ void __launch_bounds__(MAX_THREADS, 2) rms_norm_long_kernel(const Nor
         #pragma unroll
         for(int j = 0; j < 8; j++) sum += h[j] * h[j];
     }
-    const float f = inverse_root(block_sum(sum, part) / float(cols) + a.eps);
+    const float f = inverse_rms<T>(block_sum(sum, part[0]), a, row, part[1]);
     for(int c0 = first; c0 < cols; c0 += stride) {
         float h[8], g[8];
         Row8<T, KIND> w;

@@ -288,7 +288,8 @@ enum { DLP_GATE_NONE = 0, DLP_GATE_SILU = 1, DLP_GATE_GELU = 2 };
 
 /* Root-mean-square norm of each row, with a residual added before it:
  *     h = x + residual;   total = h;   y = h / sqrt(mean(h^2) + eps) * weight.
- * h is fp32 throughout; only what is stored is rounded. */
+ * h is fp32 throughout; only what is stored is rounded.  Rows of finite h have the result of the formula whatever their size, also where the squares are
+ * beyond fp32. */
 typedef struct dlp_rms_norm_args {
     const void *x;              /* [rows, cols] of `type` (fp32, fp16 or bf16) */
     const void *residual;       /* the same, or NULL */
