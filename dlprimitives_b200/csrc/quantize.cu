@@ -169,7 +169,7 @@ dlp_status launch_rows(const QuantArgs &a, bool off, cudaStream_t stream)
     const int groups = ceil_div(a.cols, 256 * ROW_PIECES);
     int log2 = 0;
     while((1 << log2) < std::min(groups, ROW_WARPS)) log2++;
-    const int blocks = ceil_div(a.rows, ROW_WARPS >> log2);
+    const int blocks = int(ceil_div<long long>(a.rows, ROW_WARPS >> log2));      // (rows may be up to 2^31 - 1)
     // few rows: more blocks to a row, until the GPU is full
     const int across = std::max(1, std::min(ceil_div(groups, 1 << log2), sm_count() * 4 / blocks));
     const dim3 grid(blocks, across);
