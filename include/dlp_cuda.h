@@ -276,8 +276,10 @@ DLP_API dlp_status dlp_batchnorm_inference_fwd(const float *x, float *y, int bat
  * are neither read nor written.
  *
  * The 8-bit form of a matrix: e4m3 numbers and an fp32 scale for each block, value = number * scale, with
- * scale = max(largest magnitude / 448, 2^-126) and number = value / scale rounded to the nearest (ties to even).  A block with a NaN or
- * an infinity has a scale that is NaN or infinite, so that what is computed from it is not finite either.  Blocks are
+ * scale = max(largest magnitude / 448, 2^-126) and number = value / scale, both in fp32, rounded to the nearest e4m3 (ties to even).  A block with
+ * a NaN or an infinity has a scale that is NaN or infinite, so that sums and products computed from it are not finite either.  (An activation may make
+ * them finite: relu and relu6 turn a NaN into 0, as everywhere in this library, and relu6, sigmoid and tanh give their bounds for an infinity.)
+ * Blocks are
  *   - 128 consecutive columns of one row (left operands): scale of block b of row r at scales[b * scale_stride + r], scale_stride >= rows;
  *   - 128 x 128 (weights): scale of row block i, column block b at scales[i * scale_stride + b], scale_stride >= number of column blocks.
  * The last block of a row, or of the rows, may be short.  An 8-bit matrix that is an operand of dlp_scaled_ip_fwd has rows on 16-byte
