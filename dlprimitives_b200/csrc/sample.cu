@@ -6,7 +6,8 @@
 //
 // Which class it is hangs on sums of up to a few hundred thousand masses, compared with a border.  Masses are whole numbers here,
 // round(w 2^b) with 63 - log2(classes) bits: their sums are exact in any order, so the result depends neither on timing nor on how
-// a row is shared out.
+// a row is shared out.  A sum is off by up to half a unit, 2^-(b+1) of the largest mass, for each class in it; classes under half a unit
+// have no mass.
 //
 // A row is read a few times, from memory once and then from L2, by a cluster of 1 to 8 blocks (so that few rows use the whole GPU); the
 // blocks gather what each has found through distributed shared memory and all come to the same conclusions.

@@ -340,7 +340,9 @@ DLP_API dlp_status dlp_scaled_ip_fwd(const dlp_scaled_ip_args *args, void *strea
  * the kept ones exceeds u times their whole mass.
  * A temperature that is not positive means the largest logit, the lowest index of equal ones; k <= 0 or >= classes, p >= 1 and m <= 0 keep
  * everything; m above 1 counts as 1.  A logit of -inf or NaN is never drawn; a row of nothing else gives -1.  Logits of +inf share the whole
- * mass.  Masses are summed as whole numbers of at least 41 bits, so the result depends neither on timing nor on the order of sums. */
+ * mass.  Masses are summed as whole numbers, in units of 2^-b of the largest one with b = min(51, 63 - ceil(log2(classes))), so the result depends
+ * neither on timing nor on the order of sums.  A sum is off by up to half a unit for each class in it, classes * 2^-(b+1) in all (2^-30 of the largest mass at
+ * 131072 classes, 2^-20 at 2^22); a class of less than half a unit is never drawn. */
 #define DLP_SAMPLE_MAX_CLASSES (1 << 22)
 typedef struct dlp_sample_args {
     const void *logits;         /* [rows, classes] of `type` (fp32, fp16 or bf16) */
