@@ -438,7 +438,9 @@ class _Torch:
     def load(cls):
         import torch
         cls.f32, cls.e4m3, cls.i32 = torch.float32, torch.float8_e4m3fn, torch.int32
-        cls.current_device, cls.raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+        # (the functions below torch's public ones, 0.09 and 0.05 us for 0.2 and 1.25; the public ones where a torch has no such functions)
+        cls.current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+        cls.raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda device: torch.cuda.current_stream(device).cuda_stream)
         cls.codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.float8_e4m3fn: 3}
 
 
