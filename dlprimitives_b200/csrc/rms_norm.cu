@@ -3,9 +3,10 @@
 // A block of threads has a row in its registers between the sum of squares and the outputs, so that a row is read once (up to 32768 columns; longer
 // ones are read a second time, from L2).  What bounds it is memory: 8192 x 5120 bf16 with residual and 8-bit output take 52 us, 5.7 TB/s of the
 // 6.5 that a copy reaches (82 us before a row stayed in registers and the next one's loads were under way, 60 before the arithmetic went two values to an
-// instruction); 8192 x 4096 fp32 without a residual 40 us, 4.2 TB/s (45 with the weights kept, for which there are no registers).  Rows off 16-byte
-// boundaries are read element by element, a warp's 32 at a time, and then it is the number of loads: 4000 x 5001 bf16 41 us, 3.5 TB/s, fp32 47, 6.0.
-// 1500 x 15001 62 us (68 in 512 threads).  One row of 4096: 2.3 us, the launch.
+// instruction); 8192 x 4096 fp32 without a residual, 8-bit output, 39 us, 4.3 TB/s (45 with the weights kept, for which there are no registers: 36 bytes a
+// thread are spilled as it is, and 760 in fp32 rows of 16385 to 32768).  Rows off 16-byte boundaries are read element by element, a warp's 32 at a
+// time, and then it is the number of loads: 4000 x 5001 with residual and 8-bit output bf16 41 us, 3.4 TB/s, fp32 49, 5.3.  1500 x 15001 63 us (68 in 512
+// threads).  One row of 4096: 1.8 us, the launch.
 #include "block8.cuh"
 
 namespace dlp {

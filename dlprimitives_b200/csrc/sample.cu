@@ -5,7 +5,7 @@
 // class drawn is the first one in index order whose running mass over the kept ones exceeds u times their whole mass.
 //
 // Which class it is hangs on sums of up to a few hundred thousand masses, compared with a border.  Masses are whole numbers here,
-// round(w 2^b) with 63 - log2(classes) bits: their sums are exact in any order, so the result depends neither on timing nor on how
+// round(w 2^b), b = min(51, 63 - log2(classes) rounded up): their sums are exact in any order, so the result depends neither on timing nor on how
 // a row is shared out.  A sum is off by up to half a unit, 2^-(b+1) of the largest mass, for each class in it; classes under half a unit
 // have no mass.
 //
@@ -19,8 +19,9 @@
 //     further as long as it holds more than 512 classes.  Then the masses of the kept classes are summed by
 //     segments of the row, and the one segment that the random number points into is gone through.
 //
-// Measured (captured): one row of 32000 with k up to 300 16.3 us, 64 rows of 128000 bf16 without settings 32, with top-p 75, 256 rows of 150001 fp32 with
-// settings of their own 137.  Memory is not what bounds it (they are 128 KB, 16 MB and 154 MB): one row is a chain of barriers, short sorts and first
+// Measured (captured): one row of 32000 with top-p and k of 50 9.5 us, of 200 15.7, of 300 (no small k any more) 44, top-p alone 25, neither 9.5, greedy 4.0; 64 rows of
+// 128000 bf16 without settings 32, with top-p 75, 256 rows of 150001 fp32 with settings of their own 137.  Two blocks of 512 threads on an SM leave 64
+// registers, under which some are spilled (16-bit logits 140 bytes stored and 268 loaded a thread, fp32 272 and 380).  Memory is not what bounds it (they are 128 KB, 16 MB and 154 MB): one row is a chain of barriers, short sorts and first
 // fetches of code, 7500 cycles up to the k-th largest, 5500 to collect, 13000 for the list; many rows are masses (about 30 instructions to a
 // class, 17000 cycles for 64000 on an SM) and sums over bins (two atomic additions to a class, 25000).  Tried: masses of fp32 pairs, within 2^-30, a tenth
 // less on rows without settings, nothing on the others; halves of the bins in arrays of their own, and barriers that a block only waits for when it

@@ -13,8 +13,8 @@
 // Every wait is bounded.
 //
 // What bounds it: an accumulator goes round by MMA, commit to both SMs, the read of tensor memory, an arrival at the leader and the next issue, and four
-// of them do not hide all of that; on large products the card's power limit takes over.  8192 rows, 4096 -> 24576: 770 to 830 us (2.0 to
-// 2.1 PFLOP/s) in short series, 945 (1.75) in long ones at 990 W and 1.57 GHz.  What it came from, same product, us: 1736 with arrivals that released
+// of them do not hide all of that: a block of K of a tile of 256 outputs takes 820 cycles, of which its MMAs are 512.  8192 rows, 4096 -> 24576: 765 to 830 us (2.0 to
+// 2.15 PFLOP/s) in short series, 945 (1.75) in long ones, where the clock falls to 1.57 GHz at 990 W.  What it came from, same product, us: 1736 with arrivals that released
 // the thread's other memory operations, too; 841 without, 804 with the scales through shared memory; 812 to 922 with accumulators of 256 columns, two
 // of them, measured in turn with this form.
 #define DLP_INLINE_WAITS
@@ -63,8 +63,9 @@ __device__ __forceinline__ void commit_pair(uint32_t bar)
 {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((unsigned short)3) : "memory");
 }
-// Relaxed: what it says is that tensor memory has been read, which the tcgen05 fence before it orders.  A release would wait for the scale copies
-// that the thread has under way (1000 cycles a block of K).
+// Relaxed: what it says is that tensor memory has been read, and that is complete: every lane has waited for its loads, and the tcgen05 fence and the warp's
+// barrier come before it.  No other memory is handed over.  A release to the cluster is a fence of all that the thread did before, at each arrival: 8192 rows,
+// 4096 -> 24576 1487 us with it, 765 without, 1024 rows 214 and 110.
 __device__ __forceinline__ void arrive_at(bool mine, uint32_t remote)
 {
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t@p mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n\t}" ::"r"(remote), "r"(uint32_t(mine)) : "memory");

@@ -319,7 +319,8 @@ DLP_API dlp_status dlp_quantize_fwd(const dlp_quantize_args *args, void *stream)
 
 /* InnerProduct of 8-bit operands, on the tensor cores:
  *     y[rows, outputs] = act(x[rows, inputs] * w[outputs, inputs]^T + bias[outputs]).
- * Products are summed in fp32.  The result does not depend on timing. */
+ * Products are summed in fp32, block by block of K, each block's sum times the product of its two scales in fp32 (which has to be in its range, and loses
+ * bits under 2^-126).  The result does not depend on timing. */
 typedef struct dlp_scaled_ip_args {
     const void *x;              /* [rows, inputs], e4m3 in blocks of one row; 16-byte aligned, x_stride a multiple of 16 */
     const float *x_scales;
