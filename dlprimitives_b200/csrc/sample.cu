@@ -612,9 +612,13 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(const SampleArgs a)
                 }
                 if(low >> G == hi >> G) break;
             }
+            // Bins end between numbers: of the 2^G keys with the same high bits the first is a number's if it is positive, the last if it is negative.
+            // So hi goes up to the last of its 2^G, or, where that is a number and hi is not, down to the last before them: no number comes into the range,
+            // and none leaves it.
+            if(!(hi & 0x80000000u) && (~hi & ((1u << G) - 1))) hi -= 1u << G;
+            hi |= (1u << G) - 1;
             int bits = G;
             while((hi - low) >> bits >= BINS) bits++;
-            hi |= (1u << G) - 1;                             // (bins end between numbers)
             histogram(low, hi, bits);
             b = find_bin(masses, left, mass_before, count_before);
             mass += mass_before;
